@@ -114,6 +114,12 @@ _SIGS = {
     'hmf_bn_bwd_reduce': (C.c_int, [_VP] * 5 + [C.c_int] * 3 + [_VP, _VP]),
     'hmf_bn_bwd_finalize': (C.c_int, [_VP, C.c_int, C.c_int] + [_VP] * 9),
     'hmf_bn_bwd_apply': (C.c_int, [_VP] * 8 + [C.c_int] * 3 + [_VP]),
+    'hmf_act8_pack': (C.c_int, [_VP, C.c_longlong, C.c_int, C.c_int, C.c_int, _VP, _VP, _VP]),
+    'hmf_act8_unpack': (C.c_int, [_VP, _VP, C.c_int, C.c_int, _VP, C.c_int, _VP]),
+    'hmf_bn_apply_act8': (C.c_int, [_VP] * 10 + [C.c_int] * 3 + [_VP]),
+    'hmf_act8_restore_activation': (C.c_int, [_VP] * 6 + [C.c_int] * 2 + [_VP]),
+    'hmf_bn_backward_act8_workspace_bytes': (C.c_size_t, [C.c_int] * 2),
+    'hmf_bn_backward_act8': (C.c_int, [_VP] * 11 + [C.c_int] * 2 + [_VP, C.c_size_t, _VP]),
     'hmf_maxpool3x3s2_nhwc_backward': (C.c_int, [_VP] * 3 + [C.c_int] * 4 + [_VP]),
     'hmf_bn_relu_maxpool3x3s2_nhwc': (C.c_int, [_VP] * 5 + [C.c_int] * 4 + [_VP]),
     'hmf_bn_relu_maxpool3x3s2_nhwc_bwd_reduce': (C.c_int, [_VP] * 6 + [C.c_int] * 4 + [_VP, _VP]),
@@ -266,6 +272,27 @@ def dptr(t):
         return None
     assert t.is_contiguous()
     return t.data_ptr()
+
+
+class on_device:
+    """`with on_device(dev):` -- dev is the current device inside, and the value is dev's current stream as the C entry points take it.  The device is
+    switched only where it differs: a guard of torch.cuda.device costs as much host time as a small launch."""
+    __slots__ = ('guard', 'index')
+
+    def __init__(self, device):
+        import torch
+        cur = torch.cuda.current_device()
+        self.index = cur if device.index is None else device.index
+        self.guard = None if self.index == cur else torch.cuda.device(self.index)
+
+    def __enter__(self):
+        import torch
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        return self.guard.__exit__(*exc) if self.guard is not None else False
 
 
 def current_stream():

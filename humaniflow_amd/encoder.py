@@ -97,6 +97,7 @@ class ResNetEncoder(nn.Module):
     # downsample branch's bias is added to the block's last bias so that branch needs no pass of its own.
     fuse_stem_pool = True    # stem convolution + max-pool as one launch (hmf_stem_conv_pool / hmf_stem_wino_pool)
     patch_s2_cfg = 8210      # tiling of the stride-2 3x3 layers (hmf_conv_patch): 8210 = 64-channel slabs, 8211 = 32-channel slabs (half the LDS)
+    activation_checkpoint = None      # training: 'int8' keeps the activations of the backward pass as 8-bit checkpoints (act8.py) instead of in 32 bits
     stem_polyphase = True    # the stem as a polyphase fast convolution (csrc/stem_wino.hip: 100 instead of 196 products per 2 x 2 outputs and channel,
                              # F(2,3)-class arithmetic); False: the direct form (csrc/stem_conv.hip)
     fuse_pairs = True        # a bottleneck's last 1x1 + the next bottleneck's first 1x1 as one launch where built (hmf_conv_pair: layer1 / layer2)

@@ -19,12 +19,16 @@ models/resnet.py).  One `torch.autograd.Function` spans the whole encoder, so no
                                            the identity branch's gradient rides in that launch's residual epilogue
   max-pool: hmf_maxpool3x3s2_nhwc / hmf_maxpool3x3s2_nhwc_backward; global average pool: torch mean / broadcast (B x C values).
 Filter re-layouts (flip, transpose, channels_last) are small torch copies per step (the filters total 45-94 MB).
+
+With `ResNetEncoder.activation_checkpoint = 'int8'` a unit keeps its y as an 8-bit checkpoint and one ReLU bit per element (act8.py) and, where an identity was
+added, its out as a second one, instead of both in 32 bits: the BatchNorm backward reads the checkpoint (hmf_bn_backward_act8), the weight gradient's input is
+rebuilt from it one unit at a time.  The forward's values are the same; the gradients carry the 8-bit rounding of what was kept.
 """
 import os
 
 import torch
 
-from . import _lib
+from . import _lib, act8
 
 CL = torch.channels_last
 WINOGRAD_WGRAD = True          # stride-1 3x3 weight gradients on hmf_conv_wgrad_winograd where the shape is built (False: hmf_conv_wgrad everywhere)
@@ -200,7 +204,38 @@ class _ZeroPool:
 
 
 class _Saved:
-    __slots__ = ('conv', 'bn', 'x', 'y', 'out', 'mean', 'rstd', 'relu', 'stride', 'stem', 'pooled', 'argmax')
+    __slots__ = ('conv', 'bn', 'x', 'y', 'out', 'mean', 'rstd', 'relu', 'stride', 'stem', 'pooled', 'argmax', 'ck', 'bits')
+
+
+def _rows_of(t):
+    """(B, C, H, W) channels_last -> its rows (B H W, C), a view."""
+    return t.permute(0, 2, 3, 1).reshape(-1, t.shape[1])
+
+
+def _map_of(rows, shape):
+    B, C, H, W = shape
+    return rows.view(B, H, W, C).permute(0, 3, 1, 2)
+
+
+class _Kept:
+    """A unit's input kept in 8 bits: `shape` for whoever asks only that, tensor() rebuilds it in 32 bits (held until drop(): the first unit of a block and
+    its downsample branch read the same one)."""
+    __slots__ = ('shape', 'ck', 'affine', '_t')
+
+    def __init__(self, shape, ck, affine=None):
+        self.shape, self.ck, self.affine, self._t = torch.Size(shape), ck, affine, None      # affine = (scale, shift, bits) of a unit without identity
+
+    def tensor(self):
+        if self._t is None:
+            self._t = _map_of(act8.unpack(self.ck) if self.affine is None else act8.restore_activation(self.ck, *self.affine), self.shape)
+        return self._t
+
+    def drop(self):
+        self._t = None
+
+
+def _input_of(s):
+    return s.x.tensor() if isinstance(s.x, _Kept) else s.x
 
 
 # The stem's bn1 -> relu -> maxpool as one pass over the convolution's output (hmf_bn_relu_maxpool3x3s2_nhwc) with a two-pass backward: the activated
@@ -208,10 +243,8 @@ class _Saved:
 STEM_TAIL_FUSED = os.environ.get('HMF_STEM_TAIL', '1') != '0'
 
 
-def _bn_forward(y, bn, residual, relu, pool=None, tracked=None, fuse_maxpool=False):
-    """Training-mode BatchNorm on the NHWC rows of y, running statistics updated in place.  Returns (out, mean, rstd).
-    pool: _ZeroPool for the fp64 sums; tracked: list collecting num_batches_tracked tensors for ONE batched increment by the caller.
-    fuse_maxpool: returns ((pooled, argmax), mean, rstd) instead -- relu(bn(y)) max-pooled 3x3 / 2 / pad 1 without materialising it."""
+def _bn_statistics(y, bn, pool, tracked):
+    """Batch statistics of the NHWC rows of y, running statistics updated in place: (mean, rstd, scale, shift)."""
     lib = _lib.load()
     B, C, H, W = y.shape
     M = B * H * W
@@ -235,6 +268,19 @@ def _bn_forward(y, bn, residual, relu, pool=None, tracked=None, fuse_maxpool=Fal
             tracked.append(bn.num_batches_tracked)
         else:
             bn.num_batches_tracked += 1
+    return mean, rstd, scale, shift
+
+
+def _bn_forward(y, bn, residual, relu, pool=None, tracked=None, fuse_maxpool=False):
+    """Training-mode BatchNorm on the NHWC rows of y, running statistics updated in place.  Returns (out, mean, rstd).
+    pool: _ZeroPool for the fp64 sums; tracked: list collecting num_batches_tracked tensors for ONE batched increment by the caller.
+    fuse_maxpool: returns ((pooled, argmax), mean, rstd) instead -- relu(bn(y)) max-pooled 3x3 / 2 / pad 1 without materialising it."""
+    lib = _lib.load()
+    B, C, H, W = y.shape
+    M = B * H * W
+    dev = y.device
+    mean, rstd, scale, shift = _bn_statistics(y, bn, pool, tracked)
+    st = _lib.current_stream()
     if fuse_maxpool:
         assert relu and residual is None
         OH, OW = (H - 1) // 2 + 1, (W - 1) // 2 + 1
@@ -252,23 +298,27 @@ def _bn_forward(y, bn, residual, relu, pool=None, tracked=None, fuse_maxpool=Fal
 def _bn_pool_backward(g, s, pool=None):
     """Backward of the fused stem tail: g = dL/d pooled map -> (gy = dL/d conv output, d gamma, d beta)."""
     lib = _lib.load()
-    B, C, H, W = s.y.shape
+    y = s.y if s.ck is None else s.y.tensor()
+    B, C, H, W = y.shape
     dev = g.device
     st = _lib.current_stream()
     acc = pool.take(C) if pool is not None else torch.zeros(2, C, dtype=torch.float64, device=dev)
-    _lib.check(lib.hmf_bn_relu_maxpool3x3s2_nhwc_bwd_reduce(g.data_ptr(), s.argmax.data_ptr(), s.pooled.data_ptr(), s.y.data_ptr(), s.mean.data_ptr(),
+    _lib.check(lib.hmf_bn_relu_maxpool3x3s2_nhwc_bwd_reduce(g.data_ptr(), s.argmax.data_ptr(), s.pooled.data_ptr(), y.data_ptr(), s.mean.data_ptr(),
                                                             s.rstd.data_ptr(), B, H, W, C, acc.data_ptr(), st), 'hmf_bn_relu_maxpool3x3s2_nhwc_bwd_reduce')
     gg, gb, ca, cb, cc = (torch.empty(C, dtype=torch.float32, device=dev) for _ in range(5))
     _lib.check(lib.hmf_bn_bwd_finalize(acc.data_ptr(), B * H * W, C, s.bn.weight.data_ptr(), s.mean.data_ptr(), s.rstd.data_ptr(), gg.data_ptr(), gb.data_ptr(),
                                        ca.data_ptr(), cb.data_ptr(), cc.data_ptr(), st), 'hmf_bn_bwd_finalize')
     gy = _cl_empty(B, C, H, W, dev)
-    _lib.check(lib.hmf_bn_relu_maxpool3x3s2_nhwc_bwd_apply(g.data_ptr(), s.argmax.data_ptr(), s.pooled.data_ptr(), s.y.data_ptr(), ca.data_ptr(), cb.data_ptr(),
+    _lib.check(lib.hmf_bn_relu_maxpool3x3s2_nhwc_bwd_apply(g.data_ptr(), s.argmax.data_ptr(), s.pooled.data_ptr(), y.data_ptr(), ca.data_ptr(), cb.data_ptr(),
                                                            cc.data_ptr(), gy.data_ptr(), B, H, W, C, st), 'hmf_bn_relu_maxpool3x3s2_nhwc_bwd_apply')
     return gy, gg, gb
 
 
 def _bn_backward(g, s, want_gz, pool=None):
     """g = dL/d out of unit s -> (gy = dL/d conv output, gz or None, d gamma, d beta)."""
+    if s.ck is not None:
+        gy, gz, gg, gb = act8.bn_backward(_rows_of(g), s.ck, s.bits, s.mean, s.rstd, s.bn.weight.detach(), want_gz)
+        return _map_of(gy, g.shape), _map_of(gz, g.shape) if want_gz else None, gg, gb
     lib = _lib.load()
     B, C, H, W = s.y.shape
     M = B * H * W
@@ -298,15 +348,16 @@ def _wgrad(gy, s):
         _lib.check(lib.hmf_conv_wgrad(gy.data_ptr(), s.x.data_ptr(), dw.data_ptr(), B, H, W, Cin, Cout, ks, s.stride, 1, _lib.current_stream()), 'hmf_conv_wgrad')
         return dw
     B, _, H, W = s.x.shape
+    x = _input_of(s)
     if ks == 3 and s.stride == 1 and WINOGRAD_WGRAD and lib.hmf_conv_wgrad_winograd_supported(H, W, Cin, Cout):
         # stride-1 3x3 layers: Winograd F(3x3, 2x2) weight gradient, written in the parameter's (Cout, Cin, 3, 3) layout (no permute pass)
         dw = torch.empty(Cout, Cin, 3, 3, dtype=torch.float32, device=gy.device)
         ws = torch.empty(int(lib.hmf_conv_wgrad_winograd_workspace_floats(Cin, Cout)), dtype=torch.float32, device=gy.device)
-        _lib.check(lib.hmf_conv_wgrad_winograd(gy.data_ptr(), s.x.data_ptr(), dw.data_ptr(), ws.data_ptr(), B, H, W, Cin, Cout, _lib.current_stream()),
+        _lib.check(lib.hmf_conv_wgrad_winograd(gy.data_ptr(), x.data_ptr(), dw.data_ptr(), ws.data_ptr(), B, H, W, Cin, Cout, _lib.current_stream()),
                    'hmf_conv_wgrad_winograd')
         return dw
     dw = torch.empty(Cout, ks, ks, Cin, dtype=torch.float32, device=gy.device)
-    _lib.check(lib.hmf_conv_wgrad(gy.data_ptr(), s.x.data_ptr(), dw.data_ptr(), B, H, W, Cin, Cout, ks, s.stride, 0, _lib.current_stream()), 'hmf_conv_wgrad')
+    _lib.check(lib.hmf_conv_wgrad(gy.data_ptr(), x.data_ptr(), dw.data_ptr(), B, H, W, Cin, Cout, ks, s.stride, 0, _lib.current_stream()), 'hmf_conv_wgrad')
     return dw.permute(0, 3, 1, 2).contiguous()
 
 
@@ -405,10 +456,15 @@ class EncoderTrainFn(torch.autograd.Function):
         dev = x.device
         saved = []
         pool, tracked = _ZeroPool(enc, dev), []
+        if enc.activation_checkpoint not in (None, 'int8'):
+            raise ValueError("humaniflow_amd: activation_checkpoint must be None or 'int8', got %r" % (enc.activation_checkpoint,))
+        keep8 = enc.activation_checkpoint == 'int8'
 
-        def unit(conv, bn, xin, relu, residual=None, stem=False):
+        def unit(conv, bn, xin, kept, relu, residual=None, stem=False):
+            """xin: the input map, kept: what the unit keeps of it for the backward pass -> (output map, what its readers keep of that)."""
             s = _Saved()
-            s.conv, s.bn, s.x, s.relu, s.stride, s.stem = conv, bn, xin, relu, conv.stride[0], stem
+            s.conv, s.bn, s.x, s.relu, s.stride, s.stem = conv, bn, kept, relu, conv.stride[0], stem
+            s.ck = s.bits = None
             if stem:
                 B, C, H, W = xin.shape
                 OH, OW = (H - 1) // 2 + 1, (W - 1) // 2 + 1
@@ -426,42 +482,54 @@ class EncoderTrainFn(torch.autograd.Function):
             if stem and STEM_TAIL_FUSED and s.y.shape[1] % 64 == 0:
                 (s.pooled, s.argmax), s.mean, s.rstd = _bn_forward(s.y, bn, None, True, pool, tracked, fuse_maxpool=True)
                 s.out = None
+                if keep8:                                             # the largest map of the network; the pooled one stays: it is layer1's input and the mask
+                    s.ck = act8.pack(_rows_of(s.y))
+                    s.y = _Kept(s.y.shape, s.ck)
                 saved.append(s)
-                return s.pooled
+                return s.pooled, s.pooled
+            if keep8 and not stem:
+                s.mean, s.rstd, scale, shift = _bn_statistics(s.y, bn, pool, tracked)
+                shape = s.y.shape
+                out, s.ck, s.bits, ck_out = act8.bn_apply(_rows_of(s.y), scale, shift, None if residual is None else _rows_of(residual), relu,
+                                                          keep_out=residual is not None)
+                s.y = s.out = None
+                saved.append(s)
+                return _map_of(out, shape), _Kept(shape, ck_out) if residual is not None else _Kept(shape, s.ck, (scale, shift, s.bits))
             s.out, s.mean, s.rstd = _bn_forward(s.y, bn, residual, relu, pool, tracked)
             saved.append(s)
-            return s.out
+            return s.out, s.out
 
         with torch.cuda.device(dev), torch.no_grad():
             _pack_all_winograd(enc, dev)
             xin = x.detach().float().contiguous()
-            a0 = unit(enc.conv1, enc.bn1, xin, True, stem=True)
+            a0, _ = unit(enc.conv1, enc.bn1, xin, xin, True, stem=True)
             if saved[0].pooled is not None:                           # bn1 + relu + maxpool in one pass: `a0` is already the pooled map
                 p0, a0 = a0, None
             else:
                 B, C, H, W = a0.shape
                 p0 = _cl_empty(B, C, (H - 1) // 2 + 1, (W - 1) // 2 + 1, dev)
                 _lib.check(lib.hmf_maxpool3x3s2_nhwc(a0.data_ptr(), p0.data_ptr(), B, H, W, C, _lib.current_stream()), 'hmf_maxpool3x3s2_nhwc')
-            cur = p0
+            cur = kept = p0
             plan = []
             for li in range(1, 5):
                 for blk in getattr(enc, 'layer%d' % li):
                     first = len(saved)
                     idt = cur
                     if blk.downsample is not None:
-                        idt = unit(blk.downsample[0], blk.downsample[1], cur, False)
-                    h = cur
+                        idt, _ = unit(blk.downsample[0], blk.downsample[1], cur, kept, False)
+                    h, kh = cur, kept
                     st = blk.stages()
                     for conv, bn in st[:-1]:
-                        h = unit(conv, bn, h, True)
+                        h, kh = unit(conv, bn, h, kh, True)
                     conv, bn = st[-1]
-                    cur = unit(conv, bn, h, True, residual=idt)
+                    cur, kept = unit(conv, bn, h, kh, True, residual=idt)
                     plan.append((first, len(saved), blk.downsample is not None))
             feats = cur.mean(dim=(2, 3))
             if tracked:
                 import ctypes as C
                 _lib.check(lib.hmf_i64_increment_batch((C.c_void_p * len(tracked))(*[t.data_ptr() for t in tracked]), len(tracked), _lib.current_stream()),
                            'hmf_i64_increment_batch')
+        ctx.keep8 = keep8
         ctx.enc, ctx.saved, ctx.plan, ctx.a0, ctx.final_shape = enc, saved, plan, a0, tuple(cur.shape)
         ctx.param_ids = [id(p) for p in params]
         # backward reads the LIVE conv / BatchNorm weights (input-gradient filters, BN coefficients): remember their versions so that an in-place
@@ -481,7 +549,9 @@ class EncoderTrainFn(torch.autograd.Function):
             if p._version != v:
                 raise RuntimeError('humaniflow_amd: an encoder parameter was modified in place between the forward and the backward of the training '
                                    'graph (version %d -> %d); the backward reads the live weights' % (v, p._version))
-        enc, saved, plan = ctx.enc, ctx.saved, ctx.plan
+        enc, saved, plan, keep8 = ctx.enc, ctx.saved, ctx.plan, ctx.keep8
+        if keep8:                                                     # the list below is emptied block by block
+            ctx.saved = None
         grads = {}
         dev = g_feats.device
         with torch.cuda.device(dev), torch.no_grad():
@@ -522,6 +592,11 @@ class EncoderTrainFn(torch.autograd.Function):
                     grads[id(ds.conv.weight)] = wgrad(gy, ds)
                     g_h = _dgrad(gy, ds, residual=g_h)
                 g = g_h
+                if keep8 and not wgrad.on:                            # what this block held is not read again (by another stream it may still be)
+                    for k in range(first, last):
+                        if isinstance(saved[k].x, _Kept):
+                            saved[k].x.drop()
+                        saved[k] = None
             # max-pool and stem
             s = saved[0]
             if s.pooled is not None:

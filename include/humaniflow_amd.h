@@ -598,6 +598,31 @@ int hmf_bn_bwd_finalize(const double* acc, int M, int C, const float* gamma, con
                         float* ca, float* cb, float* cc, void* stream);
 int hmf_bn_bwd_apply(const float* g, const float* out, const float* y, const float* ca, const float* cb, const float* cc, float* gy, float* gz_out,
                      int M, int C, int relu, void* stream);
+/* 8-bit activation checkpoints: what a training step keeps of an activation between its forward and its backward pass (1.03 bytes per element).
+ * Rows x (M, C) in blocks of 32 consecutive rows of one column:
+ *   exps  uint8 [ceil(M/32)][C]   E = exponent field of the block's largest finite magnitude (+ 1 where that would round to 128 steps), in [7, 254];
+ *                                 step = 2^(E - 133)
+ *   codes int8  [M][C]            x / step rounded to nearest even, |code| <= 127; -128 = the value was not finite (restored as NaN)
+ *   bits  uint32 [ceil(M/32)][C]  bit i of word t: the ReLU's input was > 0 in row 32 t + i
+ * |x - code step| <= step / 2 <= amax / 127 of the block (magnitudes under 2^-120 keep an absolute error of 2^-127).
+ * hmf_act8_pack reads rows of pitch ld elements (float32, or bfloat16 with bf16 != 0), any M, C >= 0 and alignment; hmf_act8_unpack writes the values,
+ * contiguous.  16-byte aligned rows of a multiple of 4 (8 bfloat16) columns move 16 bytes per lane. */
+int hmf_act8_pack(const void* x, long long ld, int bf16, int M, int C, signed char* codes, unsigned char* exps, void* stream);
+int hmf_act8_unpack(const signed char* codes, const unsigned char* exps, int M, int C, void* x, int bf16, void* stream);
+/* hmf_bn_apply that also leaves the checkpoint of y (codes, exps), the ReLU's bits (with relu, else NULL) and, with out_codes / out_exps, the checkpoint
+ * of out behind, in one pass: out = relu?(fma(y, scale, shift) (+ residual)).  C % 64 == 0; float tensors and bits 16-byte aligned. */
+int hmf_bn_apply_act8(const float* y, const float* scale, const float* shift, const float* residual, float* out, signed char* codes, unsigned char* exps,
+                      unsigned int* bits, signed char* out_codes, unsigned char* out_exps, int M, int C, int relu, void* stream);
+/* The activation behind a unit without residual, from the checkpoint of y: x = bit ? max(fma(yq, scale, shift), 0) : 0 (bits NULL: the affine alone). */
+int hmf_act8_restore_activation(const signed char* codes, const unsigned char* exps, const unsigned int* bits, const float* scale, const float* shift, float* x,
+                                int M, int C, void* stream);
+/* BatchNorm (+ ReLU) backward from the checkpoint: gz = bit ? g : 0 (bits NULL: g), xhat = (yq - mean) rstd, g_beta = sum gz, g_gamma = sum gz xhat,
+ * gy = gamma rstd (gz - g_beta / M - xhat g_gamma / M); gz is written if not NULL (the identity branch's gradient).  Sums in 64 bits in a fixed order.
+ * C % 64 == 0; the workspace (hmf_bn_backward_act8_workspace_bytes, 16-byte aligned) holds partial sums and needs no initialisation. */
+size_t hmf_bn_backward_act8_workspace_bytes(int M, int C);
+int hmf_bn_backward_act8(const float* g, const signed char* codes, const unsigned char* exps, const unsigned int* bits, const float* mean, const float* rstd,
+                         const float* gamma, float* gy, float* gz, float* g_gamma, float* g_beta, int M, int C, void* workspace, size_t workspace_bytes,
+                         void* stream);
 /* Backward of hmf_maxpool3x3s2_nhwc: x (B,H,W,C) the pooled tensor's input, g_out (B,OH,OW,C) -> g_x; ties go to the first maximum in
  * (kh, kw) scan order, as torch's forward records them.                                                                               */
 int hmf_maxpool3x3s2_nhwc_backward(const float* x, const float* g_out, float* g_x, int B, int H, int W, int C, void* stream);
