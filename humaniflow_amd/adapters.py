@@ -1,0 +1,180 @@
+"""Low-rank adapters of many requests beside a shared projection: one trained model, a small difference to its heads for every subject, camera or data set.
+
+    y[m] = W x[m] + b + s_l B_l A_l x[m],   l = ids[m]   (negative: no adapter)
+
+    y = adapted_linear(x, weight, bias, A, B, scale, ids)                        differentiable w.r.t. x, A and B (the shared projection is held fixed)
+    y, t = adapted_linear_forward(...);  dx, dA, dB = adapted_linear_backward(dy, x, t, weight, A, B, scale, ids)
+
+x (M, K), weight (N, K), bias (N) or None, A (L, r, K), B (L, N, r): all float32 or all bfloat16; scale (L) float32; ids (M) int32 / int64; r <= 64.  An id of L or
+more has no adapter to go with: that row's outputs are NaN.  The backward pass takes x as it was or as an 8-bit checkpoint (act8.Act8).
+`LowRankAdapters` holds the adapters of a HumaniflowModel's heads (models/humaniflow_model.py:232-252): `model.attach_adapters(...)`, then
+`model(..., adapter_ids=ids)`.  Kernels: csrc/adapters.hip.
+"""
+import torch
+from torch import nn
+
+from . import _lib, act8
+
+MAX_RANK = 64
+
+
+def _check(x, weight, bias, A, B, scale, ids):
+    """Shapes, types and devices -> (M, K, N, r, L, ids as int32)."""
+    dt = weight.dtype
+    if dt not in (torch.float32, torch.bfloat16):
+        raise ValueError('humaniflow_amd: adapted_linear is built for float32 and bfloat16, got %s' % dt)
+    if weight.dim() != 2 or A.dim() != 3 or B.dim() != 3 or len(x.shape) != 2:
+        raise ValueError('humaniflow_amd: adapted_linear takes x (M, K), weight (N, K), A (L, r, K), B (L, N, r); got %s, %s, %s, %s'
+                         % (tuple(x.shape), tuple(weight.shape), tuple(A.shape), tuple(B.shape)))
+    M, K = x.shape
+    N = weight.shape[0]
+    L, r = A.shape[:2]
+    if weight.shape[1] != K or A.shape[2] != K or B.shape != (L, N, r) or L < 1 or r < 1 or K < 1 or N < 1:
+        raise ValueError('humaniflow_amd: adapted_linear: x %s, weight %s, A %s, B %s do not fit' % (tuple(x.shape), tuple(weight.shape), tuple(A.shape), tuple(B.shape)))
+    if r > MAX_RANK:
+        raise ValueError('humaniflow_amd: adapters of rank %d: built up to %d' % (r, MAX_RANK))
+    if A.dtype != dt or B.dtype != dt or (bias is not None and (bias.dtype != dt or tuple(bias.shape) != (N,))):
+        raise ValueError('humaniflow_amd: adapted_linear: bias (%d), A and B must have the weight\'s type %s' % (N, dt))
+    if scale.dtype != torch.float32 or tuple(scale.shape) != (L,):
+        raise ValueError('humaniflow_amd: `scale` must be float32 (%d), got %s %s' % (L, scale.dtype, tuple(scale.shape)))
+    if ids.dtype not in (torch.int32, torch.int64) or tuple(ids.shape) != (M,):
+        raise ValueError('humaniflow_amd: `ids` must be int32 or int64 (%d), got %s %s' % (M, ids.dtype, tuple(ids.shape)))
+    _lib.require_cuda(weight, 'weight')
+    dev = weight.device
+    for name, t in (('x', x), ('bias', bias), ('A', A), ('B', B), ('scale', scale), ('ids', ids)):
+        if t is not None and t.device != dev:
+            raise ValueError('humaniflow_amd: `%s` is on %s, the weight on %s' % (name, t.device, dev))
+    if ids.dtype == torch.int64:
+        ids = ids.clamp(-1, 0x7fffffff).to(torch.int32)                  # what does not fit 32 bits stays out of range
+    return M, K, N, r, L, ids.contiguous()
+
+
+def _dense(t):
+    return None if t is None else t.detach().contiguous()
+
+
+def _rows(x):
+    """x with consecutive columns (rows may have a pitch) and that pitch."""
+    x = x.detach()
+    M, K = x.shape
+    if (K > 1 and x.stride(1) != 1) or (M > 1 and x.stride(0) < K):
+        x = x.contiguous()
+    return x, x.stride(0) if M > 1 else K
+
+
+def adapted_linear_forward(x, weight, bias, A, B, scale, ids):
+    """(y (M, N), t (M, r) float32): t = s_l A_l x is what the backward pass takes."""
+    M, K, N, r, L, ids = _check(x, weight, bias, A, B, scale, ids)
+    if x.dtype != weight.dtype:
+        raise ValueError('humaniflow_amd: adapted_linear: x is %s, the weight %s' % (x.dtype, weight.dtype))
+    x, ldx = _rows(x)
+    weight, bias, A, B, scale = _dense(weight), _dense(bias), _dense(A), _dense(B), _dense(scale)
+    dev = weight.device
+    y = torch.empty((M, N), dtype=weight.dtype, device=dev)
+    t = torch.empty((M, r), dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    n = lib.hmf_adapted_linear_workspace_bytes(M, K, N, r, L)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev) as st:
+        _lib.check(lib.hmf_adapted_linear(x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(),
+                                          ids.data_ptr(), M, K, N, r, L, int(weight.dtype == torch.bfloat16), y.data_ptr(), t.data_ptr(), ws.data_ptr(), n, st),
+                   'hmf_adapted_linear')
+    return y, t
+
+
+def adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=True):
+    """(dL/dx or None, dL/dA, dL/dB) from dy = dL/dy; x: the forward's input or its 8-bit checkpoint; t: what the forward returned."""
+    kept = x.codes if isinstance(x, act8.Act8) else x
+    M, K, N, r, L, ids = _check(kept, weight, None, A, B, scale, ids)
+    dt, dev = weight.dtype, weight.device
+    if not isinstance(x, act8.Act8) and x.dtype != dt:
+        raise ValueError('humaniflow_amd: adapted_linear: x is %s, the weight %s' % (x.dtype, dt))
+    if dy.dtype != dt or tuple(dy.shape) != (M, N) or dy.device != dev:
+        raise ValueError('humaniflow_amd: `dy` must be %s (%d, %d) on %s, got %s %s on %s' % (dt, M, N, dev, dy.dtype, tuple(dy.shape), dy.device))
+    if t.dtype != torch.float32 or tuple(t.shape) != (M, r) or t.device != dev:
+        raise ValueError('humaniflow_amd: `t` must be float32 (%d, %d) on %s, got %s %s on %s' % (M, r, dev, t.dtype, tuple(t.shape), t.device))
+    dy, t, weight, A, B, scale = _dense(dy), _dense(t), _dense(weight), _dense(A), _dense(B), _dense(scale)
+    if M == 0:
+        return (torch.empty((0, K), dtype=dt, device=dev) if need_dx else None), torch.zeros_like(A), torch.zeros_like(B)
+    if isinstance(x, act8.Act8):
+        xp, ldx, exps = x.codes, K, x.exps
+    else:
+        xp, ldx = _rows(x)
+        exps = None
+    dx = torch.empty((M, K), dtype=dt, device=dev) if need_dx else None
+    dA, dB = torch.empty_like(A), torch.empty_like(B)
+    lib = _lib.load()
+    bf16 = int(dt == torch.bfloat16)
+    n = lib.hmf_adapted_linear_backward_workspace_bytes(M, K, N, r, L, bf16)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev) as st:
+        _lib.check(lib.hmf_adapted_linear_backward(dy.data_ptr(), xp.data_ptr(), ldx, None if exps is None else exps.data_ptr(), t.data_ptr(), weight.data_ptr(),
+                                                   A.data_ptr(), B.data_ptr(), scale.data_ptr(), ids.data_ptr(), M, K, N, r, L, bf16,
+                                                   None if dx is None else dx.data_ptr(), dA.data_ptr(), dB.data_ptr(), ws.data_ptr(), n, st),
+                   'hmf_adapted_linear_backward')
+    return dx, dA, dB
+
+
+class _AdaptedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, A, B, scale, ids, checkpoint):
+        y, t = adapted_linear_forward(x, weight, bias, A, B, scale, ids)
+        x = x.detach()
+        if checkpoint == 'int8':                                         # x itself is not kept
+            ck = act8.pack(x)
+            ctx.save_for_backward(ck.codes, ck.exps, t, weight, A, B, scale, ids)
+        else:
+            ctx.save_for_backward(x, None, t, weight, A, B, scale, ids)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, exps, t, weight, A, B, scale, ids = ctx.saved_tensors
+        if exps is not None:
+            x = act8.Act8(x, exps)
+        dx, dA, dB = adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=ctx.needs_input_grad[0])
+        return dx, None, None, dA, dB, None, None, None
+
+
+def adapted_linear(x, weight, bias, A, B, scale, ids, checkpoint=None):
+    """y (M, N).  Differentiable w.r.t. x, A and B; the shared projection is held fixed (a weight, bias or scale that requires a gradient is refused).
+    checkpoint='int8': the backward pass keeps x in 8 bits."""
+    if checkpoint not in (None, 'int8'):
+        raise ValueError("humaniflow_amd: checkpoint must be None or 'int8', got %r" % (checkpoint,))
+    if torch.is_grad_enabled():
+        if weight.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad):
+            raise RuntimeError('humaniflow_amd: adapters are fitted beside a fixed projection: call requires_grad_(False) on its weight and bias, and on scale')
+        if x.requires_grad or A.requires_grad or B.requires_grad:
+            return _AdaptedLinear.apply(x, weight, bias, A, B, scale, ids, checkpoint)
+    return adapted_linear_forward(x, weight, bias, A, B, scale, ids)[0]
+
+
+class LowRankAdapters(nn.Module):
+    """Adapters of the heads of a HumaniflowModel: parameters `<layer>_A` (L, r, in) and `<layer>_B` (L, out, r) for each of `layers`, one shared factor
+    alpha / r.  A starts as the linear layers do, B at zero: an untrained adapter changes nothing.  checkpoint='int8': fitting keeps the layers' inputs in 8 bits."""
+    HEADS = ('fc1', 'fc_cam', 'fc_glob', 'fc_shape')
+
+    def __init__(self, model, num_adapters, rank, alpha=None, layers=HEADS, checkpoint=None):
+        super().__init__()
+        if checkpoint not in (None, 'int8'):
+            raise ValueError("humaniflow_amd: checkpoint must be None or 'int8', got %r" % (checkpoint,))
+        if num_adapters < 1 or not 1 <= rank <= MAX_RANK:
+            raise ValueError('humaniflow_amd: %d adapters of rank %d: at least one, of rank 1 to %d' % (num_adapters, rank, MAX_RANK))
+        unknown = [n for n in layers if n not in self.HEADS]
+        if unknown or not layers:
+            raise ValueError('humaniflow_amd: adapters go with %s, not %s' % (', '.join(self.HEADS), unknown))
+        self.num_adapters, self.rank, self.layers, self.checkpoint = num_adapters, rank, tuple(layers), checkpoint
+        ref = model.fc1.weight
+        self.register_buffer('scale', torch.full((num_adapters,), float(rank if alpha is None else alpha) / rank, dtype=torch.float32, device=ref.device))
+        for name in self.layers:
+            lin = getattr(model, name)
+            A = torch.empty(num_adapters, rank, lin.in_features, dtype=torch.float32, device=ref.device).uniform_(-1, 1) / lin.in_features ** 0.5
+            self.register_parameter(name + '_A', nn.Parameter(A))
+            self.register_parameter(name + '_B', nn.Parameter(torch.zeros(num_adapters, lin.out_features, rank, dtype=torch.float32, device=ref.device)))
+
+    def linear(self, name, lin, x, ids):
+        """lin(x) with the rows' own adapters, or lin(x) alone for a layer that has none."""
+        if name not in self.layers:
+            return torch.nn.functional.linear(x, lin.weight, lin.bias)
+        return adapted_linear(x, lin.weight, lin.bias, getattr(self, name + '_A'), getattr(self, name + '_B'), self.scale, ids, self.checkpoint)

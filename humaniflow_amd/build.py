@@ -13,7 +13,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
-SOURCES = ['so3_kernels.hip', 'smpl_kernels.hip', 'flow_pack.hip', 'flow_kernels.hip', 'flow_grad.hip', 'flow_generic.hip', 'proxy_kernels.hip', 'encoder_train.hip', 'act8.hip', 'conv_wgrad_wino.hip', 'conv_dgrad_s2.hip', 'conv_igemm.hip', 'conv_gemm.hip', 'conv_gemm_split.hip', 'conv_pair.hip', 'conv_patch.hip', 'conv_winograd.hip', 'stem_conv.hip', 'stem_wino.hip', 'train_loss.hip', 'eval_kernels.hip', 'heads_kernels.hip']
+SOURCES = ['so3_kernels.hip', 'smpl_kernels.hip', 'flow_pack.hip', 'flow_kernels.hip', 'flow_grad.hip', 'flow_generic.hip', 'proxy_kernels.hip', 'encoder_train.hip', 'act8.hip', 'adapters.hip', 'conv_wgrad_wino.hip', 'conv_dgrad_s2.hip', 'conv_igemm.hip', 'conv_gemm.hip', 'conv_gemm_split.hip', 'conv_pair.hip', 'conv_patch.hip', 'conv_winograd.hip', 'stem_conv.hip', 'stem_wino.hip', 'train_loss.hip', 'eval_kernels.hip', 'heads_kernels.hip']
 # compiled only into tools/libhumaniflow_amd_experiments.so (--experiments): measured negative results kept for their probes, not product code
 EXPERIMENT_SOURCES = ['conv_winograd_nw.hip']
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith('.h')) + ['../../include/humaniflow_amd.h', '../../include/humaniflow_amd_experiments.h']

@@ -198,6 +198,7 @@ class HumaniflowModel(nn.Module):
             raise ValueError('NUM_RESNET_LAYERS must be 18 or 50')
         self.input_feats_dim = input_feats_dim
 
+        self.adapters = None              # adapters.LowRankAdapters of the heads (attach_adapters)
         self.activation = nn.ELU()
         self.fc1 = nn.Linear(input_feats_dim, fc1_dim)
         self.fc_shape = nn.Linear(fc1_dim, self.num_shape_params * 2)
@@ -632,16 +633,32 @@ class HumaniflowModel(nn.Module):
         (losses/humaniflow_loss.py:30-31): ctx (B,23,64), R (B,23,3,3) -> (B,23) fp32, one launch (and one backward launch)."""
         return self.log_prob_parts(ctx, R, 0, self.num_bodyparts)
 
+    # ---- adapters ----
+    def attach_adapters(self, adapters):
+        """Low-rank adapters of the heads (adapters.LowRankAdapters), used by forward(adapter_ids=...); None takes them off again.  They join parameters() and, under
+        `adapters.`, state_dict(): attach them after loading a checkpoint that has none."""
+        if adapters is not None:
+            for name in adapters.layers:
+                lin, A, B = getattr(self, name), getattr(adapters, name + '_A'), getattr(adapters, name + '_B')
+                if A.shape[2] != lin.in_features or B.shape[1] != lin.out_features:
+                    raise ValueError('humaniflow_amd: adapters of %s (%d -> %d) do not fit this model (%d -> %d)'
+                                     % (name, A.shape[2], B.shape[1], lin.in_features, lin.out_features))
+        self.adapters = adapters
+
     # ---- forward ----------------------------------------------------------------------------------------------------
     def forward(self, input, compute_point_est=True, num_samples=0, use_shape_mode_for_samples=False, compute_for_loglik=False,
                 shape_for_loglik=None, pose_R_for_loglik=None, glob_R_for_loglik=None, input_feats=None,
-                grad_for_pose_point_est=False, return_input_feats=False, return_input_feats_only=False, noise=None):
+                grad_for_pose_point_est=False, return_input_feats=False, return_input_feats_only=False, noise=None, adapter_ids=None):
         """models/humaniflow_model.py:188-340.  Extra keyword `noise` = {'shape': (N,B,nb), 'pose': (23,B,N,3)} standard-normal
         tensors injects the base noise (exact-parity tests); otherwise it is drawn from the device generator in the reference's
         order (shape first, then the body parts).  Under autograd (training, train/train_humaniflow.py:248-256) the returned samples,
         shape samples and log-likelihood objects are differentiable; the point estimate is not, exactly as in the reference
         (`torch.set_grad_enabled(grad_for_pose_point_est)`, :294) unless grad_for_pose_point_est=True (round 6: its rotations join the graph through the sample
-        chain's reverse sweep at zero base noise; `pose_axisangle_point_est` stays detached)."""
+        chain's reverse sweep at zero base noise; `pose_axisangle_point_est` stays detached).
+        Extra keyword `adapter_ids` (B,) int: which of the attached low-rank adapters (attach_adapters) each image's heads use, negative = none; without it
+        attached adapters are left out."""
+        if adapter_ids is not None and getattr(self, 'adapters', None) is None:
+            raise RuntimeError('humaniflow_amd: adapter_ids given, but the model has no adapters (attach_adapters)')
         if input_feats is None:
             _lib.require_cuda(input, 'input')
             input_feats = self.image_encoder(input)
@@ -661,7 +678,15 @@ class HumaniflowModel(nn.Module):
         lib = _lib.load()
         nb, P, N = self.num_shape_params, self.num_bodyparts, int(num_samples)
 
-        if (grad and self.heads_kernel and batch_size <= 128 and isinstance(self.activation, torch.nn.ELU) and self._heads_kernel_supports(input_feats)):
+        if adapter_ids is not None:                                                      # :232-253 with every image's own adapters (adapters.py)
+            head = lambda name, v: self.adapters.linear(name, getattr(self, name), v, adapter_ids)
+            x = self.activation(head('fc1', input_feats.to(torch.float32)))
+            cam = head('fc_cam', x) + self.init_cam
+            glob_R = rot6d_to_rotmat(head('fc_glob', x) + self.init_glob)
+            shape_params = head('fc_shape', x)
+            shape_mode, shape_log_std = shape_params[:, :nb], shape_params[:, nb:]
+            shape_std = torch.exp(shape_log_std)
+        elif (grad and self.heads_kernel and batch_size <= 128 and isinstance(self.activation, torch.nn.ELU) and self._heads_kernel_supports(input_feats)):
             from .autograd import HeadsTrain                                             # :232-253 under autograd: library kernels forward and backward
             cam, glob_R, shape_mode, shape_log_std = HeadsTrain.apply(input_feats, self.fc1.weight, self.fc1.bias, self.fc_cam.weight, self.fc_cam.bias,
                                                                       self.fc_glob.weight, self.fc_glob.bias, self.fc_shape.weight, self.fc_shape.bias,
