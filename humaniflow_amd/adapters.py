@@ -73,7 +73,7 @@ def adapted_linear_forward(x, weight, bias, A, B, scale, ids):
     y = torch.empty((M, N), dtype=weight.dtype, device=dev)
     t = torch.empty((M, r), dtype=torch.float32, device=dev)
     lib = _lib.load()
-    n = lib.hmf_adapted_linear_workspace_bytes(M, K, N, r, L)
+    n = lib.hmf_adapted_linear_workspace_bytes(M, K, N, r, L, int(weight.dtype == torch.bfloat16))
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev) as st:
         _lib.check(lib.hmf_adapted_linear(x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(),
@@ -93,7 +93,10 @@ def adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=True):
         raise ValueError('humaniflow_amd: `dy` must be %s (%d, %d) on %s, got %s %s on %s' % (dt, M, N, dev, dy.dtype, tuple(dy.shape), dy.device))
     if t.dtype != torch.float32 or tuple(t.shape) != (M, r) or t.device != dev:
         raise ValueError('humaniflow_amd: `t` must be float32 (%d, %d) on %s, got %s %s on %s' % (M, r, dev, t.dtype, tuple(t.shape), t.device))
-    dy, t, weight, A, B, scale = _dense(dy), _dense(t), _dense(weight), _dense(A), _dense(B), _dense(scale)
+    dy = _dense(dy)
+    if dy.data_ptr() % 16:
+        dy = dy.clone()
+    t, weight, A, B, scale = _dense(t), _dense(weight), _dense(A), _dense(B), _dense(scale)
     if M == 0:
         return (torch.empty((0, K), dtype=dt, device=dev) if need_dx else None), torch.zeros_like(A), torch.zeros_like(B)
     if isinstance(x, act8.Act8):

@@ -15,6 +15,7 @@
 // Everything is accumulated in 32 bits.  bfloat16 operands of the many-row form are exact; t and u enter it as a high and a low bfloat16 (16 bits of mantissa),
 // so the adapters' part loses nothing against the output's own rounding.
 #include <algorithm>
+#include <type_traits>
 #include "hmf_common.h"
 
 namespace hmf {
@@ -222,9 +223,9 @@ __global__ __launch_bounds__(256) void k_ad_join(const AdArgs<T> a) {
 
 // ---------------------------------------------------------------------------------------------------
 // gradients of the adapters: G[j][c] = sum over an adapter's rows of p[m][j] z[m][c], p (M, r) in 32 bits;  dA: p = u, z = x (or its 8-bit checkpoint);  dB^T: p = t, z = dy.
-// A work-group owns (adapter, piece of <= 256 of its rows, 128 columns); its waves take a quarter of the rows each, 2 rows per MFMA step, and every lane the four
-// columns 4 i .. 4 i + 3 (one vector load feeds four MFMA tiles); they meet in LDS in a fixed order.  More pieces than one: partial sums in the workspace,
-// joined by k_ad_grad_join.
+// A work-group owns (adapter, piece of <= 256 of its rows, 128 columns); its waves take a quarter of the rows each, 4 rows per 16 x 16 x 4 MFMA step, and every lane the
+// eight columns 8 i .. 8 i + 7 (one load of 8 to 32 bytes feeds eight MFMA tiles); they meet in LDS in a fixed order.  More pieces than one: partial sums in the
+// workspace, joined by k_ad_grad_join.  Tiles of 32 ranks (32 x 32 x 2) waste half the matrix work at the usual ranks of up to 16.
 // ---------------------------------------------------------------------------------------------------
 struct AdGrad {
     const float* p;
@@ -236,84 +237,156 @@ struct AdGrad {
     int C, trans, blocks;              // blocks: column blocks of 128
 };
 
-template <typename T> __device__ __forceinline__ f32x4 z4(const AdGrad& g, int m, int c, int n, bool vec) {
-    const T* p = (const T*)g.z + (long long)m * g.ldz + c;
-    return vec ? load4<true>(p, n) : load4<false>(p, n);
-}
-__device__ __forceinline__ f32x4 z4_act8(const AdGrad& g, int m, int c, int n, bool vec) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    const signed char* pc = (const signed char*)g.z + (long long)m * g.C + c;
-    const unsigned char* pe = g.exps + (long long)(m >> 5) * g.C + c;
-    unsigned int w = 0u, e = 0u;
-    if (vec) {
-        if (n > 0) { w = *(const unsigned int*)pc; e = *(const unsigned int*)pe; }
-    } else {
+// eight consecutive elements of a row of z, as they lie in memory; columns past C read as zero
+template <typename T, bool ACT8> struct Z8;
+template <> struct Z8<float, false> {
+    f32x4 d[2];
+    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.ldz % 4 == 0 && g.C % 8 == 0 && ((uintptr_t)g.z & 15) == 0; }
+    __device__ __forceinline__ void load(const AdGrad& g, int m, int c, bool vec) {
+        const float* p = (const float*)g.z + (long long)m * g.ldz + c;
+        if (vec) {
+            if (c < g.C) { d[0] = *(const f32x4*)p; d[1] = *(const f32x4*)(p + 4); }
+        } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < n) { w |= (unsigned)(unsigned char)pc[k] << (8 * k); e |= (unsigned)pe[k] << (8 * k); }
+            for (int k = 0; k < 8; ++k)
+                if (c + k < g.C) d[k >> 2][k & 3] = p[k];
+        }
     }
+    __device__ __forceinline__ void zero() { d[0] = d[1] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ float get(int k) const { return d[k >> 2][k & 3]; }
+};
+template <> struct Z8<bf16_t, false> {
+    u16x8 d;
+    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.ldz % 8 == 0 && g.C % 8 == 0 && ((uintptr_t)g.z & 15) == 0; }
+    __device__ __forceinline__ void load(const AdGrad& g, int m, int c, bool vec) {
+        const bf16_t* p = (const bf16_t*)g.z + (long long)m * g.ldz + c;
+        if (vec) {
+            if (c < g.C) d = *(const u16x8*)p;
+        } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int q = (int)(signed char)(w >> (8 * k));
-        const float step = __uint_as_float((unsigned)max((int)((e >> (8 * k)) & 0xffu) - 6, 0) << 23);
-        v[k] = q == -128 ? nan32() : (float)q * step;
+            for (int k = 0; k < 8; ++k)
+                if (c + k < g.C) d[k] = p[k];
+        }
     }
-    return v;
-}
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d[k] = 0;
+    }
+    __device__ __forceinline__ float get(int k) const { return up(d[k]); }
+};
+template <typename T> struct Z8<T, true> {
+    unsigned int w[2], e[2];
+    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.C % 8 == 0 && ((uintptr_t)g.z & 7) == 0 && ((uintptr_t)g.exps & 7) == 0; }
+    __device__ __forceinline__ void load(const AdGrad& g, int m, int c, bool vec) {
+        const unsigned char* pc = (const unsigned char*)g.z + (long long)m * g.C + c;
+        const unsigned char* pe = g.exps + (long long)(m >> 5) * g.C + c;
+        if (vec) {
+            if (c < g.C) {
+                const uint2 a = *(const uint2*)pc, b = *(const uint2*)pe;
+                w[0] = a.x; w[1] = a.y; e[0] = b.x; e[1] = b.y;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (c + k < g.C) { w[k >> 2] |= (unsigned)pc[k] << (8 * (k & 3)); e[k >> 2] |= (unsigned)pe[k] << (8 * (k & 3)); }
+        }
+    }
+    __device__ __forceinline__ void zero() { w[0] = w[1] = e[0] = e[1] = 0u; }
+    __device__ __forceinline__ float get(int k) const {
+        const int q = (int)(signed char)(w[k >> 2] >> (8 * (k & 3)));
+        const float step = __uint_as_float((unsigned)max((int)((e[k >> 2] >> (8 * (k & 3))) & 0xffu) - 6, 0) << 23);
+        return q == -128 ? nan32() : (float)q * step;
+    }
+};
 
+constexpr int kGradLds = 4 * 32 * 64;          // floats
 // T: type of z and of the gradients; ACT8: z is a checkpoint
 template <typename T, bool ACT8>
 __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* rows, int n, int l, long long piece, bool whole, int cb, float* red) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 31, q = lane >> 5;
-    const int c = cb * 128 + 4 * i, cn = g.C - c;
-    const int esz = ACT8 ? 1 : (int)sizeof(T);
-    const bool vec = (ACT8 ? g.C : g.ldz) % 4 == 0 && g.C % 4 == 0 && ((uintptr_t)g.z & (4 * esz - 1)) == 0 && (!ACT8 || ((uintptr_t)g.exps & 3) == 0);
-    const int quarter = ((n + 3) / 4 + 1) & ~1, r0 = wave * quarter, r1 = min(r0 + quarter, n);
-    for (int j0 = 0; j0 < r; j0 += 32) {
-        const bool jin = j0 + i < r;
-        f32x16 acc[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
+    const int c = cb * 128 + 8 * i;
+    const bool vec = Z8<T, ACT8>::aligned(g);
+    const int per = ((n + 3) / 4 + 3) & ~3, r0 = wave * per, r1 = min(r0 + per, n);
+    for (int j0 = 0; j0 < r; j0 += 16) {
+        const int j = min(j0 + i, r - 1);
+        f32x4 acc[8];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+        for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         constexpr int U = 4;
-        for (int rr = r0; rr < r1; rr += 2 * U) {
-            f32x4 zv[U];
+        for (int rr = r0; rr < r1; rr += 4 * U) {
+            Z8<T, ACT8> z[U];
             float pv[U];
 #pragma unroll
             for (int s = 0; s < U; ++s) {
-                const int at = rr + 2 * s + q;
+                const int at = rr + 4 * s + q;
                 const bool in = at < r1;
                 const int m = rows[in ? at : 0];
-                pv[s] = (in && jin) ? g.p[(long long)m * r + j0 + i] : 0.f;
-                zv[s] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (in) zv[s] = ACT8 ? z4_act8(g, m, c, cn, vec) : z4<T>(g, m, c, cn, vec);
+                pv[s] = (in && j0 + i < r) ? g.p[(long long)m * r + j] : 0.f;
+                z[s].zero();
+                if (in) z[s].load(g, m, c, vec);
             }
 #pragma unroll
             for (int s = 0; s < U; ++s)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(pv[s], zv[s][t], acc[t], 0, 0, 0);
+                for (int t = 0; t < 8; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[s], z[s].get(t), acc[t], 0, 0, 0);
         }
-        // rank 8 (e >> 2) + 4 q + (e & 3) of column 4 i + t
+        // element e of tile t: rank j0 + 4 q + e of column c + t
         __syncthreads();
-        if (wave > 0)
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 8; ++t)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) red[((wave - 1) * 64 + t * 16 + e) * 64 + lane] = acc[t][e];
+            for (int e = 0; e < 4; ++e) red[(wave * 32 + t * 4 + e) * 64 + lane] = acc[t][e];
         __syncthreads();
-        if (wave == 0) {
+        auto total = [&](int t, int e) {
+            const int at = (t * 4 + e) * 64 + lane;
+            return ((red[at] + red[at + 32 * 64]) + red[at + 64 * 64]) + red[at + 96 * 64];
+        };
+        if (whole && g.trans) {                                            // wave w: columns c + 2 w, c + 2 w + 1, four ranks each
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int j = j0 + 8 * (e >> 2) + 4 * q + (e & 3);
+            for (int t2 = 0; t2 < 2; ++t2) {
+                const int t = 2 * wave + t2, jj = j0 + 4 * q;
+                T* po = (T*)g.out + ((long long)l * g.C + c + t) * r + jj;
+                T h[4] __attribute__((aligned(16)));
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const int at = (t * 16 + e) * 64 + lane;
-                    const float v = ((acc[t][e] + red[at]) + red[64 * 64 + at]) + red[2 * 64 * 64 + at];
-                    if (j < r && t < cn) {
-                        if (!whole) g.part[(piece * r + j) * g.C + c + t] = v;
-                        else if (g.trans) down((T*)g.out + ((long long)l * g.C + c + t) * r + j, v);
-                        else down((T*)g.out + ((long long)l * r + j) * g.C + c + t, v);
+                for (int e = 0; e < 4; ++e) down(h + e, total(t, e));
+                if (c + t < g.C) {
+                    if (r % 4 == 0 && ((uintptr_t)g.out & (4 * sizeof(T) - 1)) == 0) {
+                        if (jj < r) {
+                            if (sizeof(T) == 4) *(uint4*)po = *(const uint4*)h;
+                            else *(uint2*)po = *(const uint2*)h;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (jj + e < r) po[e] = h[e];
+                    }
+                }
+            }
+        } else {                                                           // wave w: rank j0 + 4 q + w, eight columns
+            const int jj = j0 + 4 * q + wave;
+            float v[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[t] = total(t, wave);
+            if (jj < r) {
+                if (!whole) {
+                    float* po = g.part + (piece * r + jj) * g.C + c;
+#pragma unroll
+                    for (int t = 0; t < 8; ++t)
+                        if (c + t < g.C) po[t] = v[t];
+                } else {
+                    T* po = (T*)g.out + ((long long)l * r + jj) * g.C + c;
+                    T h[8] __attribute__((aligned(16)));
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) down(h + t, v[t]);
+                    if (g.C % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {
+                        if (c < g.C) {
+                            *(uint4*)po = *(const uint4*)h;
+                            if (sizeof(T) == 4) *((uint4*)po + 1) = *((const uint4*)h + 1);
+                        }
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < 8; ++t)
+                            if (c + t < g.C) po[t] = h[t];
                     }
                 }
             }
@@ -339,7 +412,7 @@ __device__ __forceinline__ int rows_of(const int* ids, int M, int l, int* rows, 
 // few rows, backward, first launch: dx's partial sums, u, dB
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_ad_few_back(const AdArgs<T> a, const AdGrad db, int tiles_o, int tiles_m) {
-    __shared__ float red[3 * 64 * 64];
+    __shared__ float red[kGradLds];
     __shared__ int rows[kFewRows], cnt[4];
     const int nb = a.dx ? tiles_o * a.ksplit * tiles_m : 0;
     int id = blockIdx.x;
@@ -362,7 +435,7 @@ __global__ __launch_bounds__(256) void k_ad_few_back(const AdArgs<T> a, const Ad
 // second launch: dx = partial sums + A_l^T u, dA
 template <typename T, bool ACT8>
 __global__ __launch_bounds__(256) void k_ad_few_back2(const AdArgs<T> a, const AdGrad da, int join_wgs) {
-    __shared__ float red[3 * 64 * 64];
+    __shared__ float red[kGradLds];
     __shared__ int rows[kFewRows], cnt[4];
     int id = blockIdx.x;
     if (id < join_wgs) {
@@ -392,94 +465,136 @@ __global__ __launch_bounds__(256) void k_ad_few_back2(const AdArgs<T> a, const A
 // ---------------------------------------------------------------------------------------------------
 // many rows
 // ---------------------------------------------------------------------------------------------------
-// order: the rows by adapter (those without one last), each adapter's in their own order;  seg[l]: where adapter l begins (seg[L]: rows without, seg[L + 1] = M).
-// Work-group l counts the rows in front of its own, then places them; nothing is shared between work-groups.
-__global__ __launch_bounds__(256) void k_ad_plan(const int* __restrict__ ids, int M, int L, int* __restrict__ order, int* __restrict__ seg) {
-    __shared__ int cnt[4];
-    const int l = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int less = 0;
-    for (int m = threadIdx.x; m < M; m += 256) {
-        const int v = ids[m], key = (v < 0 || v >= L) ? L : v;
-        less += key < l;
-    }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) less += __shfl_xor(less, d);
-    if (lane == 0) cnt[wave] = less;
-    __syncthreads();
-    int at = cnt[0] + cnt[1] + cnt[2] + cnt[3];
-    if (threadIdx.x == 0) {
-        seg[l] = at;
-        if (l == L) seg[L + 1] = M;
-    }
-    for (int m0 = 0; m0 < M; m0 += 256) {
-        const int m = m0 + threadIdx.x;
-        bool mine = false;
-        if (m < M) {
-            const int v = ids[m], key = (v < 0 || v >= L) ? L : v;
-            mine = key == l;
-        }
-        const unsigned long long b = __ballot(mine);
-        __syncthreads();
-        if (lane == 0) cnt[wave] = __popcll(b);
-        __syncthreads();
-        int base = at;
-        for (int w = 0; w < wave; ++w) base += cnt[w];
-        if (mine) order[base + __popcll(b & ((1ull << lane) - 1ull))] = m;
-        at += cnt[0] + cnt[1] + cnt[2] + cnt[3];
-    }
-}
-
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void k_ad_low(const AdArgs<T> a) { low_row<T, VEC>(a, blockIdx.x); }
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_ad_up(const AdArgs<T> a) {
-    __shared__ float red[256];
-    up_row<T>(a, blockIdx.x, red);
-}
-
-// out[b][c][r] = in[b][r][c], 32 x 32 tiles
-template <typename T>
-__global__ __launch_bounds__(256) void k_ad_transpose(const T* __restrict__ in, T* __restrict__ out, int R, int C, int tc, int tr) {
-    __shared__ T s[32][33];
-    const int id = blockIdx.x, c0 = (id % tc) * 32, r0 = (id / tc) % tr * 32;
-    const long long base = (long long)(id / (tc * tr)) * R * C;
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (r0 + y + 8 * k < R && c0 + x < C) s[y + 8 * k][x] = in[base + (long long)(r0 + y + 8 * k) * C + c0 + x];
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (c0 + y + 8 * k < C && r0 + x < R) out[base + (long long)(c0 + y + 8 * k) * R + r0 + x] = s[x][y + 8 * k];
-}
-
-// out[m][o] = sum_c in[m][c] w[o][c] (+ bias[o]) + sum_j low[m][j] v[l][o][j]: forward in = x, w = W, low = t, v = B; backward in = dy, w = W^T, low = u, v = A^T.
-template <typename T> struct AdGemm {
-    const T *in, *w, *bias, *v;
-    const float* low;
-    const int *ids, *order;
-    T* out;
-    long long ldin;
-    int M, C, O, r, L, tiles_o;
+// First launch: the rows' order by adapter, and the copies of operands that the tiles below need in another layout.
+//   order: the rows by adapter (those without one last), each adapter's in their own order; key: their ids in that order;  seg[l]: where adapter l begins (seg[L]:
+//     rows without, seg[L + 1] = M).  Work-group l counts the rows in front of its own adapter's, then places these: its sixteen waves take a range of the rows
+//     each, nothing is shared between work-groups.
+//   Copies: dst[b][r][c] (pitch ldd, columns past C zero) = src[b][r][c] or, transposed, src[b][c][r]: 64 x 64 tiles, through LDS.
+struct AdCopy {
+    const void* src;
+    void* dst;
+    long long lds_, ldd, sbs, dbs;         // row pitches and batch strides of source and destination
+    int R, C, Cp, trans, tiles, tr, tc;     // destination rows, columns, padded columns; tiles = batches * tr * tc
+};
+struct AdPrep {
+    const int* ids;
+    int *order, *key, *seg;
+    int M, L, ncopy;
+    AdCopy copy[3];
 };
 
+constexpr int kPrep = 1024;                // threads: the plan of some thousand rows is two rounds of loads, not thirty
+template <typename T>
+__global__ __launch_bounds__(kPrep) void k_ad_prep(const AdPrep a) {
+    __shared__ T s[64][65];
+    __shared__ int cnt[32];
+    int id = blockIdx.x;
+    if (id <= a.L) {
+        const int l = id, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int per = ((a.M + 15) / 16 + 63) / 64 * 64, m0 = wave * per, m1 = min(m0 + per, a.M);
+        constexpr int U = 8;
+        int less = 0, mine = 0;
+        for (int mb = m0; mb < m1; mb += 64 * U) {
+            int v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = mb + 64 * u + lane < m1 ? a.ids[mb + 64 * u + lane] : -2;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool in = mb + 64 * u + lane < m1;
+                const int key = (v[u] < 0 || v[u] >= a.L) ? a.L : v[u];
+                less += in && key < l;
+                mine += in && key == l;
+            }
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) {
+            less += __shfl_xor(less, d);
+            mine += __shfl_xor(mine, d);
+        }
+        if (lane == 0) { cnt[wave] = less; cnt[16 + wave] = mine; }
+        __syncthreads();
+        int at = 0;
+        for (int w = 0; w < 16; ++w) at += cnt[w];
+        if (threadIdx.x == 0) {
+            a.seg[l] = at;
+            if (l == a.L) a.seg[l + 1] = a.M;
+        }
+        for (int w = 0; w < wave; ++w) at += cnt[16 + w];
+        for (int mb = m0; mb < m1; mb += 64 * U) {
+            int v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = mb + 64 * u + lane < m1 ? a.ids[mb + 64 * u + lane] : -2;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int m = mb + 64 * u + lane, key = (v[u] < 0 || v[u] >= a.L) ? a.L : v[u];
+                const bool in = m < m1 && key == l;
+                const unsigned long long b = __ballot(in);
+                if (in) {
+                    const int p = at + __popcll(b & ((1ull << lane) - 1ull));
+                    a.order[p] = m;
+                    a.key[p] = v[u];
+                }
+                at += __popcll(b);
+            }
+        }
+        return;
+    }
+    id -= a.L + 1;
+    int k = 0;
+    while (k < a.ncopy && id >= a.copy[k].tiles) id -= a.copy[k++].tiles;
+    if (k >= a.ncopy) return;
+    const AdCopy& c = a.copy[k];
+    const int bt = id / (c.tr * c.tc), rest = id - bt * c.tr * c.tc, r0 = rest / c.tc * 64, c0 = rest % c.tc * 64;
+    const T* src = (const T*)c.src + bt * c.sbs;
+    T* dst = (T*)c.dst + bt * c.dbs;
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    T v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int rr = c.trans ? r0 + x : r0 + y + 16 * j, cc = c.trans ? c0 + y + 16 * j : c0 + x;
+        v[j] = (rr < c.R && cc < c.C) ? src[c.trans ? (long long)cc * c.lds_ + rr : (long long)rr * c.lds_ + cc] : (T)0;
+    }
+    if (!c.trans) {                                                        // uniform
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (r0 + y + 16 * j < c.R && c0 + x < c.Cp) dst[(long long)(r0 + y + 16 * j) * c.ldd + c0 + x] = v[j];
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[x][y + 16 * j] = v[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (r0 + y + 16 * j < c.R && c0 + x < c.Cp) dst[(long long)(r0 + y + 16 * j) * c.ldd + c0 + x] = s[y + 16 * j][x];
+}
+
+// What the two types differ in.  A chunk of the reduction is 128 bytes of a row (BK elements) in both, a fragment 16 bytes.
 template <typename T> struct Mma;
-template <> struct Mma<float> {                                            // 8 reduction elements: 4 steps of the 32 x 32 x 2 MFMA, lane half q holds 4 q .. 4 q + 3
-    static constexpr int BK = 32, G = 8, E = 4, HL = 1;                     // E: elements of 16 bytes; HL: columns of the reduction per rank
+template <> struct Mma<float> {
+    static constexpr int BK = 32, E = 4, HL = 1;                            // E: elements of 16 bytes; HL: columns of the reduction per rank
     typedef f32x4 frag;
-    static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    // 32 bytes of both operands' rows: 4 steps of the 32 x 32 x 2 MFMA, lane half q holds elements 4 q .. 4 q + 3
+    static __device__ __forceinline__ f32x16 mma32(frag a, frag b, f32x16 c) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
         return c;
     }
+    // 64 bytes: 4 steps of the 16 x 16 x 4 MFMA, lane quarter holds its 16 bytes
+    static __device__ __forceinline__ f32x4 mma16(frag a, frag b, f32x4 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
     static __device__ __forceinline__ float part(float v, int) { return v; }
 };
-template <> struct Mma<bf16_t> {                                           // 16 reduction elements: one 32 x 32 x 16 MFMA, lane half q holds 8 q .. 8 q + 7
-    static constexpr int BK = 64, G = 16, E = 8, HL = 2;
+template <> struct Mma<bf16_t> {
+    static constexpr int BK = 64, E = 8, HL = 2;
     typedef u16x8 frag;
-    static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    static __device__ __forceinline__ f32x16 mma32(frag a, frag b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 mma16(frag a, frag b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ bf16_t part(float v, int lo) {       // high half, and what it leaves
         const bf16_t h = to_bf16(v);
@@ -489,191 +604,17 @@ template <> struct Mma<bf16_t> {                                           // 16
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ bool finite(bf16_t v) { return (v & 0x7f80u) != 0x7f80u; }
 
-// 128 x 128 tile, 4 waves of 64 x 64 (2 x 2 MFMA tiles), two LDS stages of one chunk (BK reduction elements) each, rows padded by 16 bytes.  Chunks past the
-// shared weight's are the adapters': element e belongs to the tile's adapter list[e / rr], rank e % rr.  The rows of other adapters hold zeros there, and a zero
-// times an infinity or a NaN of a weight would reach them: such weights are staged as zeros and added to their own rows at the end.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
-    typedef Mma<T> X;
-    typedef typename X::frag frag;
-    constexpr int BK = X::BK, E = X::E, P = BK + E;                         // pitch of an LDS row
-    constexpr int SEG = BK / E, NS = 128 * SEG / 256;                       // 16-byte pieces of a row; pieces per thread and operand
-    __shared__ __attribute__((aligned(16))) T sw[2][128 * P], sx[2][128 * P];
-    __shared__ int rowid[128], slot[128], list[128], nlist[2], odd;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 31, q = lane >> 5;
-    const int ot = blockIdx.x % a.tiles_o, mt = blockIdx.x / a.tiles_o;
-    const int o0 = ot * 128, p0 = mt * 128;
-    // the tile's rows and its distinct adapters, in order
-    if (tid == 0) odd = 0;
-    if (tid < 128) {
-        const int p = p0 + tid;
-        const int m = p < a.M ? a.order[p] : -1;
-        int l = m >= 0 ? a.ids[m] : -1;
-        if (l >= a.L) l = -1;
-        const int prev = (tid > 0 && p < a.M) ? a.ids[a.order[p - 1]] : -1;
-        const bool first = l >= 0 && l != prev;
-        const unsigned long long b = __ballot(first);
-        const int before = __popcll(b & ((2ull << lane) - 1ull));           // first rows up to and including this one
-        rowid[tid] = m;
-        if (lane == 0) nlist[wave] = __popcll(b);
-        slot[tid] = l >= 0 ? before - 1 : -1000;                            // of this wave's list; the second wave's is moved below
-        if (first) list[wave * 64 + before - 1] = l;
-    }
-    __syncthreads();
-    // the second wave's first rows may continue the first wave's last adapter: then before - 1 = -1 is that adapter's place once moved
-    const int n0 = nlist[0], n1 = nlist[1];
-    int moved = 0;
-    if (tid >= 64 && tid < 128) moved = list[tid];
-    __syncthreads();
-    if (tid >= 64 && tid < 128) {
-        if (tid - 64 < n1) list[n0 + tid - 64] = moved;
-        slot[tid] += n0;
-    }
-    __syncthreads();
-    const int rr = a.r * X::HL, ext = (n0 + n1) * rr;
-    const int kc = (a.C + BK - 1) / BK, nc = kc + (ext + BK - 1) / BK;
-
-    frag gw[NS], gx[NS];
-    auto fetch = [&](int c) {
-        if (c < kc) {
-            const int cb = c * BK;
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const int e = tid + 256 * s, row = e / SEG, cc = cb + (e % SEG) * E;
-                const int o = o0 + row, m = rowid[row];
-                frag zw, zx;
-#pragma unroll
-                for (int k = 0; k < E; ++k) { zw[k] = 0; zx[k] = 0; }
-                const T* pw = a.w + (long long)o * a.C + cc;
-                const T* px = a.in + (long long)m * a.ldin + cc;
-                if (VEC) {
-                    if (o < a.O && cc < a.C) zw = *(const frag*)pw;
-                    if (m >= 0 && cc < a.C) zx = *(const frag*)px;
-                } else {
-#pragma unroll
-                    for (int k = 0; k < E; ++k) {
-                        if (o < a.O && cc + k < a.C) zw[k] = pw[k];
-                        if (m >= 0 && cc + k < a.C) zx[k] = px[k];
-                    }
-                }
-                gw[s] = zw;
-                gx[s] = zx;
-            }
-        } else {
-            const int eb = (c - kc) * BK;
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const int e = tid + 256 * s, row = e / SEG;
-                const int o = o0 + row, m = rowid[row], sl = slot[row];
-                frag zw, zx;
-#pragma unroll
-                for (int k = 0; k < E; ++k) {
-                    const int el = eb + (e % SEG) * E + k, ad = el / rr, jj = el - ad * rr, lo = jj >= a.r, j = lo ? jj - a.r : jj;
-                    zw[k] = 0;
-                    zx[k] = 0;
-                    if (el < ext) {
-                        if (o < a.O) {
-                            zw[k] = a.v[((long long)list[ad] * a.O + o) * a.r + j];
-                            if (!finite(zw[k])) { zw[k] = 0; odd = 1; }
-                        }
-                        if (ad == sl) zx[k] = X::part(a.low[(long long)m * a.r + j], lo);
-                    }
-                }
-                gw[s] = zw;
-                gx[s] = zx;
-            }
-        }
-    };
-    auto stash = [&](int b) {
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            const int e = tid + 256 * s, at = (e / SEG) * P + (e % SEG) * E;
-            *(frag*)&sw[b][at] = gw[s];
-            *(frag*)&sx[b][at] = gx[s];
-        }
-    };
-    f32x16 acc[2][2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[t][v][e] = 0.f;
-    const int wo = (wave & 1) * 64, wm = (wave >> 1) * 64;
-    fetch(0);
-    stash(0);
-    __syncthreads();
-    for (int c = 0; c < nc; ++c) {
-        const int b = c & 1;
-        if (c + 1 < nc) fetch(c + 1);
-#pragma unroll
-        for (int g = 0; g < BK / X::G; ++g) {
-            frag fw[2], fx[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                fw[t] = *(const frag*)&sw[b][(wo + 32 * t + i) * P + g * X::G + q * E];
-                fx[t] = *(const frag*)&sx[b][(wm + 32 * t + i) * P + g * X::G + q * E];
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int v = 0; v < 2; ++v) acc[t][v] = X::mma(fw[t], fx[v], acc[t][v]);
-        }
-        if (c + 1 < nc) stash(b ^ 1);
-        __syncthreads();
-    }
-    // lane (m = column i) holds outputs 8 (e >> 2) + 4 q + (e & 3): four consecutive ones per store
-    const bool vec = a.O % 4 == 0 && ((uintptr_t)a.out & (4 * sizeof(T) - 1)) == 0;
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
-        const int m = rowid[wm + 32 * v + i];
-        if (m < 0) continue;
-        const int l = a.ids[m];
-        const bool bad = l >= a.L;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e4 = 0; e4 < 4; ++e4) {
-                const int o = o0 + wo + 32 * t + 8 * e4 + 4 * q;
-                float z[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    z[e] = acc[t][v][4 * e4 + e];
-                    if (a.bias && o + e < a.O) z[e] += up(a.bias[o + e]);
-                    if (bad) z[e] = nan32();
-                    if (odd && l >= 0 && !bad && o + e < a.O)
-                        for (int j = 0; j < a.r; ++j) {
-                            const T vv = a.v[((long long)l * a.O + o + e) * a.r + j];
-                            if (!finite(vv)) z[e] = fmaf(a.low[(long long)m * a.r + j], up(vv), z[e]);
-                        }
-                }
-                T* po = a.out + (long long)m * a.O + o;
-                if (vec) {
-                    if (o < a.O) {
-                        T h[4] __attribute__((aligned(16)));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) down(h + e, z[e]);
-                        if (sizeof(T) == 4) *(uint4*)po = *(const uint4*)h;
-                        else *(uint2*)po = *(const uint2*)h;
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (o + e < a.O) down(po + e, z[e]);
-                }
-            }
-    }
-}
-
-// Piece z of the adapters' rows: adapter l has max(1, ceil(rows / kFewRows)) of them, one behind the other.  All threads return the same; l = L: no such piece.
-__device__ __forceinline__ void find_piece(const int* seg, int L, int z, int& l, int& p, int& n, int& first) {
+// Piece z of the order: segment l (of n) has max(MIN, ceil(rows / R)) pieces of R rows, one behind the other.  All lanes of a wave return the same: the segment, which of
+// its pieces this is, how many it has; l = n: no such piece.
+template <int R, int MIN>
+__device__ __forceinline__ void find_piece(const int* seg, int n, int z, int& l, int& p, int& np) {
     const int lane = threadIdx.x & 63;
     int base = 0;
-    for (int l0 = 0; l0 < L; l0 += 64) {
+    for (int l0 = 0; l0 < n; l0 += 64) {
         const int li = l0 + lane;
-        const int rows = li < L ? seg[li + 1] - seg[li] : 0;
-        const int np = li < L ? max(1, (rows + kFewRows - 1) / kFewRows) : 0;
-        int incl = np;
+        const int rows = li < n ? seg[li + 1] - seg[li] : 0;
+        const int mine = li < n ? max(MIN, (rows + R - 1) / R) : 0;
+        int incl = mine;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const int o = __shfl_up(incl, d);
@@ -683,24 +624,382 @@ __device__ __forceinline__ void find_piece(const int* seg, int L, int z, int& l,
         if (over) {
             const int k = __ffsll((long long)over) - 1;
             l = l0 + k;
-            const int np_k = __shfl(np, k);
-            first = base + __shfl(incl, k) - np_k;
-            p = z - first;
-            n = np_k;
+            np = __shfl(mine, k);
+            p = z - (base + __shfl(incl, k) - np);
             return;
         }
         base += __shfl(incl, 63);
     }
-    l = L;
-    p = n = first = 0;
+    l = n;
+    p = np = 0;
+}
+
+typedef __attribute__((address_space(3))) void* ad_lds_t;
+typedef const __attribute__((address_space(1))) void* ad_glb_t;
+// one LDS-DMA request: lane l's 16 bytes at g land at dst + 16 l
+static __device__ __forceinline__ void ad_dma16(const char* g, void* dst) { __builtin_amdgcn_global_load_lds((ad_glb_t)g, (ad_lds_t)dst, 16, 0, 0); }
+#define HMF_AD_VMCNT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
+
+// low[m][j] = s_l sum_c in[m][c] v[l][j][c]:  t (in = x, v = A) and u (in = dy, v = B^T).  A work-group owns up to 16 rows of one adapter; its sixteen waves take a
+// part of the reduction each (16 rows x 16 ranks per MFMA) and meet in LDS in a fixed order.  Operands go through LDS by DMA although nothing is used twice: the MFMA's
+// operand layout has 16 rows in 16 neighbouring lanes, and a load of 16 bytes per lane in that layout takes the address unit 64 cycles instead of 16 (4,096 rows
+// of 2,048 in bfloat16: 11.6 us, and twice that in 32 bits).  C: whole chunks.
+struct AdLow {
+    const void *in, *v;
+    const float* scale;
+    const int *order, *key, *seg;
+    float* low;
+    long long ldin, ldv;                    // row pitches; v: (L r) rows
+    int M, C, r, L;
+};
+template <typename T>
+__global__ __launch_bounds__(1024) void k_ad_low(const AdLow a) {
+    typedef Mma<T> X;
+    typedef typename X::frag frag;
+    constexpr int U = 4;                                                    // groups of 64 bytes in flight per wave and operand
+    __shared__ __attribute__((aligned(16))) char smem[16 * 2 * U * 1024];
+    float* red = (float*)smem;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, q = lane >> 4;
+    int ad, pc, np;
+    find_piece<16, 0>(a.seg, a.L + 1, blockIdx.x, ad, pc, np);              // the rows without an adapter are the last segment
+    if (ad > a.L) return;
+    ad = __builtin_amdgcn_readfirstlane(ad);
+    const int end = a.seg[ad + 1], at = a.seg[ad] + 16 * pc + i;
+    const bool live = at < end;
+    const int p = min(at, end - 1), m = a.order[p];                         // places past the segment's last row repeat it and write nothing
+    if (ad == a.L) {                                                        // no adapter: zero; an id that no adapter has: NaN
+        if (live && q == 0)
+            for (int j = wave; j < a.r; j += 16) a.low[(long long)m * a.r + j] = a.key[p] < 0 ? 0.f : nan32();
+        return;
+    }
+    const float s = a.scale[ad];
+    const int ng = a.C / (4 * X::E), per = (ng + 15) / 16, g0 = wave * per, g1 = min(g0 + per, ng);         // groups of 64 bytes
+    // DMA: lane brings piece (lane & 3) ^ s of row lane >> 2, s = (row >> 2) & 3; fragment (i, q) lies in slot q ^ s of row i
+    const int dr = lane >> 2, dc = (lane & 3) ^ ((dr >> 2) & 3);
+    const char* xr = (const char*)((const T*)a.in + (long long)__shfl(m, dr) * a.ldin) + 16 * dc;
+    char* mine = smem + wave * 2 * U * 1024;
+    const char* fr = mine + i * 64 + ((q ^ ((i >> 2) & 3)) * 16);
+    for (int j0 = 0; j0 < a.r; j0 += 16) {
+        const char* vr = (const char*)((const T*)a.v + ((long long)ad * a.r + min(j0 + dr, a.r - 1)) * a.ldv) + 16 * dc;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int g = g0; g < g1; g += U) {
+#pragma unroll
+            for (int h = 0; h < U; ++h)
+                if (g + h < g1) {                                           // wave-uniform
+                    ad_dma16(xr + (long long)(g + h) * 64, mine + h * 1024);
+                    ad_dma16(vr + (long long)(g + h) * 64, mine + (U + h) * 1024);
+                }
+            HMF_AD_VMCNT(0);
+#pragma unroll
+            for (int h = 0; h < U; ++h)
+                if (g + h < g1) acc = X::mma16(*(const frag*)(fr + (U + h) * 1024), *(const frag*)(fr + h * 1024), acc);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");               // read before the next round overwrites
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[wave * 256 + e * 64 + lane] = acc[e];
+        __syncthreads();
+        if (wave < 4) {                                                     // wave w finishes element w: rank j0 + 4 q + w of row i
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) v += red[w * 256 + tid];
+            const int j = j0 + 4 * q + wave;
+            if (live && j < a.r) a.low[(long long)m * a.r + j] = s * v;
+        }
+        __syncthreads();
+    }
+}
+
+// out[m][o] = sum_c in[m][c] w[o][c] (+ bias[o]) + sum_j low[m][j] v[l][o][j]: forward in = x, w = W, low = t, v = B; backward in = dy, w = W^T, low = u, v = A^T.
+template <typename T> struct AdGemm {
+    const T *in, *w, *bias, *v;
+    const float* low;
+    const int *order, *key;
+    T* out;
+    long long ldin, ldw, vl, vo, vj;        // pitches; strides of v
+    int M, C, O, r, L, tiles_o;             // C: whole chunks
+    float* partial;                         // with several splits of the reduction (gridDim.y): [split][M][O]
+    int per;                                // chunks of a split
+};
+
+// BT x BT tile, 4 waves of (BT / 2) x (BT / 2); a ring of 4 LDS stages of one chunk (128 bytes of every row of both operands) filled by LDS-DMA three chunks
+// ahead: with one chunk ahead through registers the 128-tile took 2.2 us a chunk, the latency of its loads.  The 16-byte slot c of row r lies at slot
+// c ^ ((r >> 1) & 7) (the DMA writes in lane order, so the source address is permuted): a fragment read hits every bank once.
+// After the shared weight's chunks come the adapters': 16-byte piece P of a row belongs to the tile's adapter list[P / pp] and holds E of its ranks (bfloat16: the
+// high halves of all ranks, then the low ones).  The rows of other adapters hold zeros there,
+// and a zero times an infinity or a NaN of a weight would reach them: such weights are staged as zeros and added to their own rows at the end.
+template <typename T, int BT>
+__global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
+    typedef Mma<T> X;
+    typedef typename X::frag frag;
+    constexpr int BK = X::BK, E = X::E, S = 4;
+    constexpr int ND = BT / 32;                                             // DMA requests of a wave, operand and chunk (8 rows each)
+    constexpr int NT = BT / 64;                                             // MFMA tiles of a wave, each way
+    constexpr int NS = BT * 8 / 256;                                        // 16-byte pieces of a thread, operand and chunk
+    constexpr int OP = BT * 128, STAGE = 2 * OP;                            // bytes
+    __shared__ __attribute__((aligned(16))) char smem[S * STAGE + (3 * BT + 4) * 4];      // one object: a second one makes hipcc wait for the DMA before every read
+    int* rowid = (int*)(smem + S * STAGE);
+    int *slot = rowid + BT, *list = slot + BT, *nlist = list + BT, *odd = nlist + 2;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 31, q = lane >> 5;
+    // XCD x (work-groups go round robin) gets a contiguous run of tiles, the tiles of one row panel next to each other
+    const int all = gridDim.x, t8 = all >> 3, id = (all & 7) ? blockIdx.x : (blockIdx.x & 7) * t8 + (blockIdx.x >> 3);
+    const int ot = id % a.tiles_o, mt = id / a.tiles_o;
+    const int o0 = ot * BT, p0 = mt * BT;
+    // the tile's rows and its distinct adapters, in order
+    if (tid == 0) *odd = 0;
+    bool first = false;
+    int l = -1, before = 0;
+    if (tid < BT) {
+        const int p = min(p0 + tid, a.M - 1), prev = max(p - 1, 0);
+        const int m = a.order[p], id = a.key[p], idp = a.key[prev];
+        const bool in = p0 + tid < a.M;
+        l = (in && id >= 0) ? (id < a.L ? id : -2) : -1;
+        first = l >= 0 && (tid == 0 || l != idp);
+        const unsigned long long b = __ballot(first);
+        before = __popcll(b & ((2ull << lane) - 1ull));                     // first rows of this wave up to and including this one
+        rowid[tid] = in ? m : -1 - m;                                       // places past the last row read it and store nothing
+        if (lane == 0) nlist[wave] = __popcll(b);
+    }
+    __syncthreads();
+    const int n0 = nlist[0], nad = n0 + (BT > 64 ? nlist[1] : 0);
+    if (tid < BT) {                                                         // a second wave's leading rows may continue the first one's last adapter: place n0 - 1
+        const int at = before - 1 + (wave > 0 ? n0 : 0);
+        slot[tid] = l >= 0 ? at : l;                                        // -1: no adapter, -2: an id that no adapter has
+        if (first) list[at] = l;
+    }
+    __syncthreads();
+    // chunks of this split; 16-byte pieces of an adapter's ranks, of an adapter, of all (the first split's), and their chunks
+    const int cfirst = blockIdx.y * a.per, kc = min(a.per, a.C / BK - cfirst);
+    const int pr = (a.r + E - 1) / E, pp = pr * X::HL, ext = blockIdx.y == 0 ? nad * pp : 0, ne = (ext + 7) / 8;
+
+    // DMA sources: request d of wave w brings rows 8 (w ND + d) .. + 7; rows that are not there read a valid one, whose results are not stored
+    const char *gw[ND], *gx[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        const int row = (wave * ND + d) * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+        gw[d] = (const char*)(a.w + (long long)min(o0 + row, a.O - 1) * a.ldw) + 16 * c + (long long)cfirst * 128;
+        const int m = rowid[row];
+        gx[d] = (const char*)(a.in + (long long)(m < 0 ? -1 - m : m) * a.ldin) + 16 * c + (long long)cfirst * 128;
+    }
+    auto issue = [&](int c, int lo, int hi) {
+        char* st = smem + (c & (S - 1)) * STAGE + wave * ND * 1024;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            if (d < lo || d >= hi) continue;
+            ad_dma16(gw[d] + (long long)c * 128, st + d * 1024);
+            ad_dma16(gx[d] + (long long)c * 128, st + OP + d * 1024);
+        }
+    };
+    // the adapters' chunks go through registers: raw values first, so that the first of them are loaded under the main loop.  A thread's pieces lie in the same column.
+    frag ew[NS];
+    float ex[NS][E];
+    const bool vec_v = a.vj == 1 && a.r % E == 0 && ((uintptr_t)a.v & 15) == 0;
+    int elo = 0;
+    auto fetch = [&](int c) {
+        const int P = c * 8 + (tid & 7), ad = P / pp, rem = P - ad * pp, j0 = (rem >= pr ? rem - pr : rem) * E;
+        elo = rem >= pr;
+        const bool live = P < ext;
+        const T* vb = a.v + (live ? (long long)list[ad] : 0ll) * a.vl + j0 * a.vj;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int row = (tid + 256 * s) >> 3, o = o0 + row;
+            const bool mine = live && slot[row] == ad;
+            const float* pl = a.low + (long long)(mine ? rowid[row] : 0) * a.r + j0;
+#pragma unroll
+            for (int k = 0; k < E; ++k) ex[s][k] = (mine && j0 + k < a.r) ? pl[k] : 0.f;
+            if (vec_v) {
+#pragma unroll
+                for (int k = 0; k < E; ++k) ew[s][k] = 0;
+                if (live && o < a.O) ew[s] = *(const frag*)(vb + (long long)o * a.vo);
+            } else {
+#pragma unroll
+                for (int k = 0; k < E; ++k) ew[s][k] = (live && o < a.O && j0 + k < a.r) ? vb[(long long)o * a.vo + k * a.vj] : (T)0;
+            }
+        }
+    };
+    auto stash = [&](int st) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int e = tid + 256 * s, row = e >> 3, at = row * 128 + (((e & 7) ^ ((row >> 1) & 7)) * 16);
+            frag zw = ew[s], zx;
+            bool ok = true;
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                ok = ok && finite(zw[k]);
+                zx[k] = X::part(ex[s][k], elo);
+            }
+            if (!ok) {
+                *odd = 1;
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (!finite(zw[k])) zw[k] = 0;
+            }
+            *(frag*)(smem + st * STAGE + at) = zw;
+            *(frag*)(smem + st * STAGE + OP + at) = zx;
+        }
+    };
+    f32x16 acc[NT][NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < NT; ++v)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[t][v][e] = 0.f;
+    const int wo = (wave & 1) * (BT / 2), wm = (wave >> 1) * (BT / 2);
+    const char *pw = smem + (wo + i) * 128, *px = smem + OP + (wm + i) * 128;
+    int go[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) go[g] = ((2 * g + q) ^ ((i >> 1) & 7)) * 16;
+    frag fw[2][NT], fx[2][NT];
+    auto frags = [&](int st, int g) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            fw[g & 1][t] = *(const frag*)(pw + st * STAGE + go[g] + t * 4096);
+            fx[g & 1][t] = *(const frag*)(px + st * STAGE + go[g] + t * 4096);
+        }
+    };
+    auto mma = [&](int g) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int v = 0; v < NT; ++v) acc[t][v] = X::mma32(fw[g & 1][t], fx[g & 1][v], acc[t][v]);
+    };
+    if (ne > 0) fetch(0);
+#pragma unroll
+    for (int c = 0; c < S - 1; ++c)
+        if (c < kc) issue(c, 0, ND);
+    // One chunk: its own fragments group by group, each read under the MFMAs of the group before; chunk c + 1 is there too (at most the one behind it is on its way),
+    // so the next chunk's first fragments are read under this one's last MFMAs and the matrix pipe does not drain at the barrier.
+    auto iteration = [&](int c, auto MORE) {
+        constexpr bool more = decltype(MORE)::value;
+        if (more) HMF_AD_VMCNT(2 * ND);
+        else HMF_AD_VMCNT(0);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int st = c & (S - 1);
+        constexpr int nm = NT * NT * (sizeof(T) == 4 ? 4 : 1);
+        auto group = [&](auto G) {
+            constexpr int g = decltype(G)::value;
+            if (g < 3) frags(st, g + 1);
+            else if (more || c + 1 < kc) frags((c + 1) & (S - 1), 0);
+            mma(g);
+            if (more && g < ND) issue(c + S - 1, g, g + 1);                 // into the stage that everybody has read (chunk c - 1)
+            // order: an MFMA on the fragments at hand, the next fragments' reads, the DMA requests, the other MFMAs (the compiler waits for all reads at once:
+            // reads issued in front of the first MFMA would be waited for there)
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * NT, 0);
+            if (more && g < ND) __builtin_amdgcn_sched_group_barrier(0x010, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, nm - 1, 0);
+        };
+        group(std::integral_constant<int, 0>{});
+        group(std::integral_constant<int, 1>{});
+        group(std::integral_constant<int, 2>{});
+        group(std::integral_constant<int, 3>{});
+    };
+    if (kc >= S - 1) HMF_AD_VMCNT(2 * 2 * ND);                              // the first chunk
+    else HMF_AD_VMCNT(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    frags(0, 0);
+    int c = 0;
+    for (; c + S - 1 < kc; ++c) iteration(c, std::true_type{});
+    for (; c < kc; ++c) iteration(c, std::false_type{});
+    auto compute = [&](int st) {
+        frags(st, 0);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (g < 3) frags(st, g + 1);
+            mma(g);
+        }
+    };
+    for (int e = 0; e < ne; ++e) {
+        __syncthreads();
+        stash(0);
+        __syncthreads();
+        if (e + 1 < ne) fetch(e + 1);
+        compute(0);
+    }
+    __syncthreads();
+    // Epilogue through LDS: lane (m = column i) holds outputs 8 (e >> 2) + 4 q + (e & 3); every wave turns its own tile round and stores 16 bytes per lane, whole rows of
+    // BT / 2 outputs.
+    const bool any_odd = *odd != 0;
+    constexpr int H = BT / 2, PF = H + 4;                                   // outputs of a wave's rows, pitch in floats
+    static_assert(4 * H * PF * 4 <= S * STAGE, "the turned tiles lie in the ring");
+    float* tw = (float*)smem + wave * H * PF;
+#pragma unroll
+    for (int v = 0; v < NT; ++v)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4)
+                *(f32x4*)(tw + (32 * v + i) * PF + 32 * t + 8 * e4 + 4 * q) = f32x4{acc[t][v][4 * e4], acc[t][v][4 * e4 + 1], acc[t][v][4 * e4 + 2], acc[t][v][4 * e4 + 3]};
+    constexpr int LPR = H / E, RPI = 64 / LPR;                              // lanes of a row, rows of an instruction
+    const int oc = (lane % LPR) * E, o = o0 + wo + oc;
+    const bool vec = a.O % E == 0 && ((uintptr_t)a.out & 15) == 0;
+    float bv[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) bv[k] = (a.bias && !a.partial && o + k < a.O) ? up(a.bias[o + k]) : 0.f;
+#pragma unroll
+    for (int s = 0; s < H / RPI; ++s) {
+        const int row = s * RPI + lane / LPR, m = rowid[wm + row];
+        float z[E];
+#pragma unroll
+        for (int k = 0; k < E; k += 4) {
+            const f32x4 u = *(const f32x4*)(tw + row * PF + oc + k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[k + e] = u[e] + bv[k + e];
+        }
+        if (m < 0 || o >= a.O) continue;
+        const int sl = slot[wm + row];
+        if (sl == -2 || any_odd) {
+            const int id = sl >= 0 ? list[sl] : -1;
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                if (sl == -2) z[k] = nan32();
+                else if (id >= 0 && o + k < a.O)
+                    for (int j = 0; j < a.r; ++j) {
+                        const T vv = a.v[id * a.vl + (o + k) * a.vo + j * a.vj];
+                        if (!finite(vv)) z[k] = fmaf(a.low[(long long)m * a.r + j], up(vv), z[k]);
+                    }
+            }
+        }
+        if (a.partial) {
+            float* pp_ = a.partial + ((long long)blockIdx.y * a.M + m) * a.O + o;
+#pragma unroll
+            for (int k = 0; k < E; ++k)
+                if (o + k < a.O) pp_[k] = z[k];
+            continue;
+        }
+        T h[E] __attribute__((aligned(16)));
+#pragma unroll
+        for (int k = 0; k < E; ++k) down(h + k, z[k]);
+        T* po = a.out + (long long)m * a.O + o;
+        if (vec) *(uint4*)po = *(const uint4*)h;
+        else
+#pragma unroll
+            for (int k = 0; k < E; ++k)
+                if (o + k < a.O) po[k] = h[k];
+    }
+}
+
+// out = the splits' sums, in order, + bias
+template <typename T>
+__global__ __launch_bounds__(256) void k_ad_sum(const float* __restrict__ partial, int splits, const T* __restrict__ bias, T* __restrict__ out, long long n, int O) {
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) {
+        float v = partial[e];
+#pragma unroll 4
+        for (int k = 1; k < splits; ++k) v += partial[(long long)k * n + e];
+        if (bias) v += up(bias[e % O]);
+        down(out + e, v);
+    }
 }
 
 template <typename T, bool ACT8>
 __global__ __launch_bounds__(256) void k_ad_grads(const AdGrad da, const AdGrad db, const int* __restrict__ order, const int* __restrict__ seg, int r, int L) {
-    __shared__ float red[3 * 64 * 64];
+    __shared__ float red[kGradLds];
     __shared__ int rows[kFewRows];
-    int l, p, np, first;
-    find_piece(seg, L, blockIdx.y, l, p, np, first);
+    int l, p, np;
+    find_piece<kFewRows, 1>(seg, L, blockIdx.y, l, p, np);
     if (l >= L) return;
     const int s0 = seg[l] + p * kFewRows, n = min(kFewRows, seg[l + 1] - s0);
     if ((int)threadIdx.x < n) rows[threadIdx.x] = order[s0 + threadIdx.x];
@@ -754,8 +1053,24 @@ static void few_split(int M, int O, int Cn, int* ksplit, int* kw) {
     *ksplit = blocks_of(Cn, 4 * *kw);
 }
 
-struct FwdWs { size_t t, partial, order, seg, total; };
-static FwdWs fwd_ws(int M, int K, int N, int r, int L) {
+// Tiles of 128 where they fill three quarters of the CUs, else of 64; where those leave CUs idle too, the reduction is split until two work-groups go on each CU, but
+// not under 8 chunks (512 rows, 2,048 -> 1,024 in 32 bits, 128 tiles: 44 us unsplit).
+static void gemm_shape(int M, int O, int Cp, size_t z, int* bt, int* splits, int* per) {
+    *bt = (long long)blocks_of(M, 128) * blocks_of(O, 128) >= 192 ? 128 : 64;
+    const int kc = (int)(Cp * z / 128), tiles = blocks_of(M, *bt) * blocks_of(O, *bt);
+    const int want = tiles >= 256 ? 1 : std::max(1, std::min(kc / 8, 512 / tiles));
+    *per = blocks_of(kc, want);
+    *splits = blocks_of(kc, *per);
+}
+static size_t gemm_partial(int M, int O, int Cp, size_t z) {
+    int bt, splits, per;
+    gemm_shape(M, O, Cp, z, &bt, &splits, &per);
+    return splits > 1 ? (size_t)splits * M * O * 4 : 0;
+}
+// the many-row form's rows: whole chunks of 128 bytes, 16-byte aligned
+static inline int padded(int C, size_t z) { const int bk = (int)(128 / z); return (C + bk - 1) / bk * bk; }
+struct FwdWs { size_t t, partial, order, key, seg, xp, wp, ap, total; };
+static FwdWs fwd_ws(int M, int K, int N, int r, int L, size_t z) {
     FwdWs w{};
     size_t o = 0;
     w.t = o; o += al((size_t)M * r * 4);
@@ -764,28 +1079,36 @@ static FwdWs fwd_ws(int M, int K, int N, int r, int L) {
         few_split(M, N, K, &ks, &kw);
         w.partial = o; o += al((size_t)ks * M * N * 4);
     } else {
+        const size_t Kp = padded(K, z);
         w.order = o; o += al((size_t)M * 4);
+        w.key = o; o += al((size_t)M * 4);
         w.seg = o; o += al((size_t)(L + 2) * 4);
+        w.xp = o; o += al(M * Kp * z);                                     // used where x, W or A is not laid out like that
+        w.wp = o; o += al(N * Kp * z);
+        w.ap = o; o += al((size_t)L * r * Kp * z);
+        w.partial = o; o += al(gemm_partial(M, N, (int)Kp, z));
     }
     w.total = o;
     return w;
 }
-struct BwdWs { size_t u, partial, order, seg, wt, at, part_a, part_b, total; };
-static BwdWs bwd_ws(int M, int K, int N, int r, int L, int bf16) {
+struct BwdWs { size_t u, partial, order, key, seg, wt, bt, dyp, part_a, part_b, total; };
+static BwdWs bwd_ws(int M, int K, int N, int r, int L, size_t z) {
     BwdWs w{};
     size_t o = 0;
-    const size_t z = bf16 ? 2 : 4;
     w.u = o; o += al((size_t)M * r * 4);
     if (M <= kFewRows) {
         int ks, kw;
         few_split(M, K, N, &ks, &kw);
         w.partial = o; o += al((size_t)ks * M * K * 4);
     } else {
-        const size_t pieces = (size_t)L + M / kFewRows;
+        const size_t pieces = (size_t)L + M / kFewRows, Np = padded(N, z);
         w.order = o; o += al((size_t)M * 4);
+        w.key = o; o += al((size_t)M * 4);
         w.seg = o; o += al((size_t)(L + 2) * 4);
-        w.wt = o; o += al((size_t)N * K * z);
-        w.at = o; o += al((size_t)L * r * K * z);
+        w.wt = o; o += al(K * Np * z);
+        w.bt = o; o += al((size_t)L * r * Np * z);
+        w.dyp = o; o += N == (int)Np ? 0 : al(M * Np * z);
+        w.partial = o; o += al(gemm_partial(M, K, (int)Np, z));
         w.part_a = o; o += al(pieces * r * K * 4);
         w.part_b = o; o += al(pieces * r * N * 4);
     }
@@ -796,15 +1119,46 @@ static BwdWs bwd_ws(int M, int K, int N, int r, int L, int bf16) {
 static int check_sizes(const char* who, int M, int K, int N, int r, int L) {
     if (M < 0 || K < 1 || N < 1 || r < 1 || L < 1) return fail(HMF_ERR_INVALID, "%s: M=%d K=%d N=%d r=%d L=%d", who, M, K, N, r, L);
     if (r > kMaxRank) return fail(HMF_ERR_UNSUPPORTED, "%s: rank %d, built up to %d", who, r, kMaxRank);
-    if (L > 65535 || M > (1 << 30) || (long long)blocks_of(M, 128) * blocks_of(std::max(N, K), 128) > 0x7fffffffLL || (long long)L + M / kFewRows > 65535)
+    const long long tk = blocks_of(K, 32) + 2, tn = blocks_of(N, 32) + 2;    // 32 x 32 tiles of the copies (padded rows)
+    if (L > 65535 || (long long)L + M / kFewRows > 65535 || (long long)L * r > 0x3fffffffLL || blocks_of(M, 32) * std::max(tk, tn) > 0x1fffffffLL || tk * tn > 0x1fffffffLL ||
+        blocks_of((long long)L * r, 32) * std::max(tk, tn) > 0x1fffffffLL || (long long)L * blocks_of(r, 32) * tn > 0x1fffffffLL)
         return fail(HMF_ERR_UNSUPPORTED, "%s: M=%d K=%d N=%d L=%d exceed the grid", who, M, K, N, L);
+    return HMF_OK;
+}
+
+static AdCopy copy_job(const void* src, void* dst, long long lds_, long long ldd, long long sbs, long long dbs, int batches, int R, int C, int Cp, int trans) {
+    AdCopy c{src, dst, lds_, ldd, sbs, dbs, R, C, Cp, trans, 0, blocks_of(R, 64), blocks_of(Cp, 64)};
+    c.tiles = batches * c.tr * c.tc;
+    return c;
+}
+template <typename T> static int prepare(const AdPrep& p, hipStream_t st) {
+    long long wgs = p.L + 1;
+    for (int k = 0; k < p.ncopy; ++k) wgs += p.copy[k].tiles;
+    hipLaunchKernelGGL(k_ad_prep<T>, dim3((unsigned)wgs), dim3(kPrep), 0, st, p);
+    HMF_LAUNCH_CHECK();
+    return HMF_OK;
+}
+template <typename T> static int gemm(AdGemm<T>& m, void* partial, hipStream_t st) {
+    int bt, splits;
+    gemm_shape(m.M, m.O, m.C, sizeof(T), &bt, &splits, &m.per);
+    m.tiles_o = blocks_of(m.O, bt);
+    m.partial = splits > 1 ? (float*)partial : nullptr;
+    const dim3 grid(m.tiles_o * blocks_of(m.M, bt), splits);
+    if (bt == 128) hipLaunchKernelGGL((k_ad_gemm<T, 128>), grid, dim3(256), 0, st, m);
+    else hipLaunchKernelGGL((k_ad_gemm<T, 64>), grid, dim3(256), 0, st, m);
+    HMF_LAUNCH_CHECK();
+    if (splits > 1) {
+        const long long n = (long long)m.M * m.O;
+        hipLaunchKernelGGL(k_ad_sum<T>, dim3((unsigned)std::min<long long>((n + 255) / 256, 4096)), dim3(256), 0, st, m.partial, splits, m.bias, m.out, n, m.O);
+        HMF_LAUNCH_CHECK();
+    }
     return HMF_OK;
 }
 
 template <typename T>
 static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const T* a, const T* b, const float* scale, const int* ids, int M, int K, int N, int r, int L,
                      T* y, float* t, char* ws, hipStream_t st) {
-    const FwdWs o = fwd_ws(M, K, N, r, L);
+    const FwdWs o = fwd_ws(M, K, N, r, L, sizeof(T));
     AdArgs<T> g{};
     g.x = x; g.ldx = ldx; g.w = w; g.bias = bias; g.a = a; g.b = b; g.scale = scale; g.ids = ids; g.y = y; g.t = t ? t : (float*)(ws + o.t);
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
@@ -822,26 +1176,39 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
         HMF_LAUNCH_CHECK();
         return HMF_OK;
     }
-    int *order = (int*)(ws + o.order), *seg = (int*)(ws + o.seg);
-    hipLaunchKernelGGL(k_ad_plan, dim3(L + 1), dim3(256), 0, st, ids, M, L, order, seg);
-    HMF_LAUNCH_CHECK();
-    if (vec) hipLaunchKernelGGL((k_ad_low<T, true>), dim3(M), dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_ad_low<T, false>), dim3(M), dim3(256), 0, st, g);
-    HMF_LAUNCH_CHECK();
+    // x, W and A as whole chunks of aligned rows: themselves, or copies
+    const int Kp = padded(K, sizeof(T));
+    AdPrep pr{};
+    pr.ids = ids; pr.order = (int*)(ws + o.order); pr.key = (int*)(ws + o.key); pr.seg = (int*)(ws + o.seg); pr.M = M; pr.L = L;
+    AdLow lo{};
+    lo.in = x; lo.ldin = ldx; lo.v = a; lo.ldv = K;
     AdGemm<T> m{};
-    m.in = x; m.ldin = ldx; m.w = w; m.bias = bias; m.v = b; m.low = g.t; m.ids = ids; m.order = order; m.out = y;
-    m.M = M; m.C = K; m.O = N; m.r = r; m.L = L; m.tiles_o = blocks_of(N, 128);
-    const dim3 grid(m.tiles_o * blocks_of(M, 128));
-    if (vec) hipLaunchKernelGGL((k_ad_gemm<T, true>), grid, dim3(256), 0, st, m);
-    else hipLaunchKernelGGL((k_ad_gemm<T, false>), grid, dim3(256), 0, st, m);
+    m.w = w; m.ldw = K;
+    if (K != Kp || ldx % V || off16(x)) {
+        pr.copy[pr.ncopy++] = copy_job(x, ws + o.xp, ldx, Kp, 0, 0, 1, M, K, Kp, 0);
+        lo.in = ws + o.xp; lo.ldin = Kp;
+    }
+    if (K != Kp || off16(w)) {
+        pr.copy[pr.ncopy++] = copy_job(w, ws + o.wp, K, Kp, 0, 0, 1, N, K, Kp, 0);
+        m.w = (const T*)(ws + o.wp); m.ldw = Kp;
+    }
+    if (K != Kp || off16(a)) {
+        pr.copy[pr.ncopy++] = copy_job(a, ws + o.ap, K, Kp, 0, 0, 1, L * r, K, Kp, 0);
+        lo.v = ws + o.ap; lo.ldv = Kp;
+    }
+    if (int rc = prepare<T>(pr, st)) return rc;
+    lo.scale = scale; lo.order = pr.order; lo.key = pr.key; lo.seg = pr.seg; lo.low = g.t; lo.M = M; lo.C = Kp; lo.r = r; lo.L = L;
+    hipLaunchKernelGGL(k_ad_low<T>, dim3(L + 1 + M / 16), dim3(1024), 0, st, lo);
     HMF_LAUNCH_CHECK();
-    return HMF_OK;
+    m.in = (const T*)lo.in; m.ldin = lo.ldin; m.bias = bias; m.v = b; m.vl = (long long)N * r; m.vo = r; m.vj = 1; m.low = g.t; m.order = pr.order; m.key = pr.key; m.out = y;
+    m.M = M; m.C = Kp; m.O = N; m.r = r; m.L = L;
+    return gemm<T>(m, ws + o.partial, st);
 }
 
 template <typename T>
 static int backward_t(const T* dy, const void* x, long long ldx, const unsigned char* exps, const float* t, const T* w, const T* a, const T* b, const float* scale,
                       const int* ids, int M, int K, int N, int r, int L, T* dx, T* da, T* db, char* ws, hipStream_t st) {
-    const BwdWs o = bwd_ws(M, K, N, r, L, sizeof(T) == 2);
+    const BwdWs o = bwd_ws(M, K, N, r, L, sizeof(T));
     AdArgs<T> g{};
     g.dy = dy; g.w = w; g.a = a; g.b = b; g.scale = scale; g.ids = ids; g.dx = dx; g.u = (float*)(ws + o.u);
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
@@ -865,26 +1232,29 @@ static int backward_t(const T* dy, const void* x, long long ldx, const unsigned 
         HMF_LAUNCH_CHECK();
         return HMF_OK;
     }
-    int *order = (int*)(ws + o.order), *seg = (int*)(ws + o.seg);
-    hipLaunchKernelGGL(k_ad_plan, dim3(L + 1), dim3(256), 0, st, ids, M, L, order, seg);
-    HMF_LAUNCH_CHECK();
-    hipLaunchKernelGGL(k_ad_up<T>, dim3(M), dim3(256), 0, st, g);
+    // W^T and B^T, dy as whole chunks of aligned rows
+    const int Np = padded(N, sizeof(T));
+    AdPrep pr{};
+    pr.ids = ids; pr.order = (int*)(ws + o.order); pr.key = (int*)(ws + o.key); pr.seg = (int*)(ws + o.seg); pr.M = M; pr.L = L;
+    pr.copy[pr.ncopy++] = copy_job(b, ws + o.bt, r, Np, (long long)N * r, (long long)r * Np, L, r, N, Np, 1);
+    if (dx) pr.copy[pr.ncopy++] = copy_job(w, ws + o.wt, K, Np, 0, 0, 1, K, N, Np, 1);
+    const T* dyp = dy;
+    if (N != Np) {
+        pr.copy[pr.ncopy++] = copy_job(dy, ws + o.dyp, N, Np, 0, 0, 1, M, N, Np, 0);
+        dyp = (const T*)(ws + o.dyp);
+    }
+    if (int rc = prepare<T>(pr, st)) return rc;
+    AdLow lo{};
+    lo.in = dyp; lo.ldin = Np; lo.v = ws + o.bt; lo.ldv = Np; lo.scale = scale; lo.order = pr.order; lo.key = pr.key; lo.seg = pr.seg; lo.low = g.u; lo.M = M; lo.C = Np; lo.r = r; lo.L = L;
+    hipLaunchKernelGGL(k_ad_low<T>, dim3(L + 1 + M / 16), dim3(1024), 0, st, lo);
     HMF_LAUNCH_CHECK();
     if (dx) {
-        T *wt = (T*)(ws + o.wt), *at = (T*)(ws + o.at);
-        const int tk = blocks_of(K, 32);
-        hipLaunchKernelGGL(k_ad_transpose<T>, dim3(tk * blocks_of(N, 32)), dim3(256), 0, st, w, wt, N, K, tk, blocks_of(N, 32));
-        HMF_LAUNCH_CHECK();
-        hipLaunchKernelGGL(k_ad_transpose<T>, dim3(tk * blocks_of(r, 32) * L), dim3(256), 0, st, a, at, r, K, tk, blocks_of(r, 32));
-        HMF_LAUNCH_CHECK();
         AdGemm<T> m{};
-        m.in = dy; m.ldin = N; m.w = wt; m.v = at; m.low = g.u; m.ids = ids; m.order = order; m.out = dx;
-        m.M = M; m.C = N; m.O = K; m.r = r; m.L = L; m.tiles_o = blocks_of(K, 128);
-        const dim3 grid(m.tiles_o * blocks_of(M, 128));
-        if (vec) hipLaunchKernelGGL((k_ad_gemm<T, true>), grid, dim3(256), 0, st, m);
-        else hipLaunchKernelGGL((k_ad_gemm<T, false>), grid, dim3(256), 0, st, m);
-        HMF_LAUNCH_CHECK();
+        m.in = dyp; m.ldin = Np; m.w = (const T*)(ws + o.wt); m.ldw = Np; m.v = a; m.vl = (long long)r * K; m.vo = 1; m.vj = K; m.low = g.u; m.order = pr.order; m.key = pr.key;
+        m.out = dx; m.M = M; m.C = Np; m.O = K; m.r = r; m.L = L;
+        if (int rc = gemm<T>(m, ws + o.partial, st)) return rc;
     }
+    const int *order = pr.order, *seg = pr.seg;
     ga.part = (float*)(ws + o.part_a);
     gb.part = (float*)(ws + o.part_b);
     const dim3 grid(ga.blocks + gb.blocks, L + M / kFewRows);
@@ -903,9 +1273,9 @@ using namespace hmf;
 
 extern "C" {
 
-size_t hmf_adapted_linear_workspace_bytes(int M, int K, int N, int r, int L) {
+size_t hmf_adapted_linear_workspace_bytes(int M, int K, int N, int r, int L, int bf16) {
     if (M < 1 || K < 1 || N < 1 || r < 1 || L < 1) return 0;
-    return fwd_ws(M, K, N, r, L).total;
+    return fwd_ws(M, K, N, r, L, bf16 ? 2 : 4).total;
 }
 
 int hmf_adapted_linear(const void* x, long long ldx, const void* w, const void* bias, const void* a, const void* b, const float* scale, const int* ids, int M, int K,
@@ -913,7 +1283,7 @@ int hmf_adapted_linear(const void* x, long long ldx, const void* w, const void* 
     if (int rc = check_sizes("hmf_adapted_linear", M, K, N, r, L)) return rc;
     if (M == 0) return HMF_OK;
     if (!x || !w || !a || !b || !scale || !ids || !y || ldx < K) return fail(HMF_ERR_INVALID, "hmf_adapted_linear: null argument or ldx=%lld < K=%d", ldx, K);
-    const size_t need = fwd_ws(M, K, N, r, L).total;
+    const size_t need = fwd_ws(M, K, N, r, L, bf16 ? 2 : 4).total;
     if (!workspace || workspace_bytes < need || off16(workspace))
         return fail(HMF_ERR_WORKSPACE, "hmf_adapted_linear: workspace %zu < %zu bytes (16-byte aligned)", workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;
@@ -926,7 +1296,7 @@ int hmf_adapted_linear(const void* x, long long ldx, const void* w, const void* 
 
 size_t hmf_adapted_linear_backward_workspace_bytes(int M, int K, int N, int r, int L, int bf16) {
     if (M < 1 || K < 1 || N < 1 || r < 1 || L < 1) return 0;
-    return bwd_ws(M, K, N, r, L, bf16).total;
+    return bwd_ws(M, K, N, r, L, bf16 ? 2 : 4).total;
 }
 
 int hmf_adapted_linear_backward(const void* dy, const void* x, long long ldx, const unsigned char* exps, const float* t, const void* w, const void* a, const void* b,
@@ -936,7 +1306,8 @@ int hmf_adapted_linear_backward(const void* dy, const void* x, long long ldx, co
     if (M < 1) return fail(HMF_ERR_INVALID, "hmf_adapted_linear_backward: no rows");
     if (!dy || !x || !t || !w || !a || !b || !scale || !ids || !da || !db || (exps ? ldx != K : ldx < K))
         return fail(HMF_ERR_INVALID, "hmf_adapted_linear_backward: null argument, or ldx=%lld with K=%d (a checkpoint is contiguous)", ldx, K);
-    const size_t need = bwd_ws(M, K, N, r, L, bf16).total;
+    if (off16(dy)) return fail(HMF_ERR_INVALID, "hmf_adapted_linear_backward: dy must be 16-byte aligned");
+    const size_t need = bwd_ws(M, K, N, r, L, bf16 ? 2 : 4).total;
     if (!workspace || workspace_bytes < need || off16(workspace))
         return fail(HMF_ERR_WORKSPACE, "hmf_adapted_linear_backward: workspace %zu < %zu bytes (16-byte aligned)", workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;

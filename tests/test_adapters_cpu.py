@@ -58,7 +58,7 @@ def test_refusals_of_the_c_entry_points(lib):
     buf = (C.c_float * 4096)()
     p = C.c_void_p((C.addressof(buf) + 15) & ~15)
     n = C.c_void_p(None)
-    need = lib.hmf_adapted_linear_workspace_bytes(4, 6, 3, 2, 2)
+    need = lib.hmf_adapted_linear_workspace_bytes(4, 6, 3, 2, 2, 0)
     fw = lambda x=p, ldx=6, M=4, K=6, N=3, r=2, L=2, ws=p, nb=1 << 20: lib.hmf_adapted_linear(x, ldx, p, n, p, p, p, p, M, K, N, r, L, 0, p, n, ws, nb, n)
     assert need > 0 and fw(M=0) == 0
     assert fw(x=n) == -1 and fw(ldx=5) == -1 and fw(K=0) == -1 and fw(M=-1) == -1 and fw(L=0) == -1 and fw(r=0) == -1
@@ -67,7 +67,7 @@ def test_refusals_of_the_c_entry_points(lib):
     need = lib.hmf_adapted_linear_backward_workspace_bytes(4, 6, 3, 2, 2, 0)
     bw = lambda dy=p, ldx=6, exps=n, M=4, r=2, ws=p, nb=1 << 20: lib.hmf_adapted_linear_backward(dy, p, ldx, exps, p, p, p, p, p, p, M, 6, 3, r, 2, 0, p, p, p, ws, nb, n)
     assert bw(dy=n) == -1 and bw(ldx=5) == -1 and bw(ldx=7, exps=p) == -1 and bw(M=0) == -1 and bw(r=65) == -2 and bw(nb=need - 1) == -4 and bw(ws=n) == -4
-    assert lib.hmf_adapted_linear_workspace_bytes(0, 6, 3, 2, 2) == 0
+    assert lib.hmf_adapted_linear_workspace_bytes(0, 6, 3, 2, 2, 0) == 0
 
 
 def test_module_layout_and_refusals():
