@@ -279,13 +279,13 @@ def dptr(t):
 
 
 class on_device:
-    """`with on_device(dev):` -- dev is the current device inside, and the value is dev's current stream as the C entry points take it.  The device is
-    switched only where it differs: a guard of torch.cuda.device costs as much host time as a small launch."""
+    """`with on_device(dev) as st:` -- dev is the current device inside, st its current stream as the C entry points take it.  The device is switched only where
+    it differs, and the stream is asked for without building a torch.cuda.Stream: a small launch's host time is mostly such things."""
     __slots__ = ('guard', 'index')
 
     def __init__(self, device):
         import torch
-        cur = torch.cuda.current_device()
+        cur = torch._C._cuda_getDevice()
         self.index = cur if device.index is None else device.index
         self.guard = None if self.index == cur else torch.cuda.device(self.index)
 
@@ -293,7 +293,7 @@ class on_device:
         import torch
         if self.guard is not None:
             self.guard.__enter__()
-        return torch.cuda.current_stream(self.index).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         return self.guard.__exit__(*exc) if self.guard is not None else False

@@ -21,8 +21,8 @@ _DTYPES = (torch.float32, torch.bfloat16)
 
 
 class Act8:
-    """Checkpoint of rows (M, C): codes int8 (M, C), exps uint8 (ceil(M / 32), C), both contiguous."""
-    __slots__ = ('codes', 'exps')
+    """Checkpoint of rows (M, C): codes int8 (M, C), exps uint8 (ceil(M / 32), C), both contiguous (pack() and bn_apply() lay them in one buffer)."""
+    __slots__ = ('shape', 'device', 'codes_ptr', 'exps_ptr', '_codes', '_exps', '_buf', '_at')
 
     def __init__(self, codes, exps):
         if codes.dtype != torch.int8 or exps.dtype != torch.uint8 or codes.dim() != 2:
@@ -32,28 +32,49 @@ class Act8:
             raise ValueError('humaniflow_amd: Act8: exps %s on %s do not fit codes %s on %s' % (tuple(exps.shape), exps.device, tuple(codes.shape), codes.device))
         if not (codes.is_contiguous() and exps.is_contiguous()):
             raise ValueError('humaniflow_amd: Act8 codes and exps must be contiguous')
-        self.codes, self.exps = codes, exps
+        self.shape, self.device, self._codes, self._exps, self._buf = codes.shape, codes.device, codes, exps, None
+        self.codes_ptr, self.exps_ptr = codes.data_ptr(), exps.data_ptr()
 
     @property
-    def shape(self):
-        return self.codes.shape
+    def codes(self):
+        if self._codes is None:
+            M, C = self.shape
+            self._codes = self._buf[self._at:self._at + M * C].view(torch.int8).view(M, C)
+        return self._codes
 
     @property
-    def device(self):
-        return self.codes.device
+    def exps(self):
+        if self._exps is None:
+            M, C = self.shape
+            at, nb = self._at + _round16(M * C), (M + BLOCK - 1) // BLOCK
+            self._exps = self._buf[at:at + nb * C].view(nb, C)
+        return self._exps
 
     def nbytes(self):
-        return self.codes.numel() + self.exps.numel()
+        M, C = self.shape
+        return M * C + (M + BLOCK - 1) // BLOCK * C
 
 
-def _new(M, C, device):
-    return (torch.empty((M, C), dtype=torch.int8, device=device), torch.empty(((M + BLOCK - 1) // BLOCK, C), dtype=torch.uint8, device=device))
+def _round16(n):
+    return (n + 15) & ~15
 
 
-def _wrap(codes, exps):
+def _bytes_of(M, C):
+    return _round16(M * C) + _round16((M + BLOCK - 1) // BLOCK * C)
+
+
+def _in_buffer(buf, at, M, C):
+    """The checkpoint of (M, C) rows whose codes and exponents lie (or will lie) at byte `at` of buf."""
     ck = Act8.__new__(Act8)
-    ck.codes, ck.exps = codes, exps
+    ck.shape, ck.device, ck._codes, ck._exps, ck._buf, ck._at = torch.Size((M, C)), buf.device, None, None, buf, at
+    ck.codes_ptr = buf.data_ptr() + at
+    ck.exps_ptr = ck.codes_ptr + _round16(M * C)
     return ck
+
+
+def _on_gpu(ck):
+    if ck.device.type != 'cuda':
+        _lib.require_cuda(ck.codes, 'codes')
 
 
 def _rows(t, name, C=None, M=None):
@@ -91,24 +112,23 @@ def pack(x):
     M, C = x.shape
     if (C > 1 and x.stride(1) != 1) or (M > 1 and x.stride(0) < C):
         x = x.contiguous()
-    codes, exps = _new(M, C, x.device)
+    ck = _in_buffer(torch.empty(_bytes_of(M, C), dtype=torch.uint8, device=x.device), 0, M, C)
     lib = _lib.load()
     with _lib.on_device(x.device) as st:
-        _lib.check(lib.hmf_act8_pack(x.data_ptr(), x.stride(0) if M > 1 else C, int(x.dtype == torch.bfloat16), M, C, codes.data_ptr(), exps.data_ptr(), st),
-                   'hmf_act8_pack')
-    return _wrap(codes, exps)
+        _lib.check(lib.hmf_act8_pack(x.data_ptr(), x.stride(0) if M > 1 else C, int(x.dtype == torch.bfloat16), M, C, ck.codes_ptr, ck.exps_ptr, st), 'hmf_act8_pack')
+    return ck
 
 
 def unpack(ck, dtype=torch.float32):
     """The values of a checkpoint as contiguous rows (M, C), float32 or bfloat16 (a code has 7 bits: exact in both)."""
     if dtype not in _DTYPES:
         raise ValueError('humaniflow_amd: act8.unpack gives float32 or bfloat16, not %s' % dtype)
-    _lib.require_cuda(ck.codes, 'codes')
-    M, C = ck.codes.shape
-    x = torch.empty((M, C), dtype=dtype, device=ck.codes.device)
+    _on_gpu(ck)
+    M, C = ck.shape
+    x = torch.empty((M, C), dtype=dtype, device=ck.device)
     lib = _lib.load()
     with _lib.on_device(x.device) as st:
-        _lib.check(lib.hmf_act8_unpack(ck.codes.data_ptr(), ck.exps.data_ptr(), M, C, x.data_ptr(), int(dtype == torch.bfloat16), st), 'hmf_act8_unpack')
+        _lib.check(lib.hmf_act8_unpack(ck.codes_ptr, ck.exps_ptr, M, C, x.data_ptr(), int(dtype == torch.bfloat16), st), 'hmf_act8_unpack')
     return x
 
 
@@ -123,29 +143,30 @@ def bn_apply(y, scale, shift, residual=None, relu=True, keep_out=False):
     dev = y.device
     _same_device(dev, scale=scale, shift=shift, residual=residual)
     out = torch.empty_like(y)
-    codes, exps = _new(M, C, dev)
-    bits = torch.empty(exps.shape, dtype=torch.int32, device=dev) if relu else None
-    oc, oe = _new(M, C, dev) if keep_out else (None, None)
+    n = _bytes_of(M, C)
+    buf = torch.empty(2 * n if keep_out else n, dtype=torch.uint8, device=dev)
+    ck, ck_out = _in_buffer(buf, 0, M, C), _in_buffer(buf, n, M, C) if keep_out else None
+    bits = torch.empty(((M + BLOCK - 1) // BLOCK, C), dtype=torch.int32, device=dev) if relu else None
     lib = _lib.load()
     with _lib.on_device(dev) as st:
         _lib.check(lib.hmf_bn_apply_act8(y.data_ptr(), scale.data_ptr(), shift.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(),
-                                         codes.data_ptr(), exps.data_ptr(), None if bits is None else bits.data_ptr(), None if oc is None else oc.data_ptr(),
-                                         None if oe is None else oe.data_ptr(), M, C, int(relu), st), 'hmf_bn_apply_act8')
-    return out, _wrap(codes, exps), bits, _wrap(oc, oe) if keep_out else None
+                                         ck.codes_ptr, ck.exps_ptr, None if bits is None else bits.data_ptr(), ck_out.codes_ptr if keep_out else None,
+                                         ck_out.exps_ptr if keep_out else None, M, C, int(relu), st), 'hmf_bn_apply_act8')
+    return out, ck, bits, ck_out
 
 
 def restore_activation(ck, scale, shift, bits=None):
     """The float32 output of a bn_apply without residual, from its checkpoint: relu(value * scale + shift), zero where the ReLU's bit is clear (bits None:
     the affine alone)."""
-    _lib.require_cuda(ck.codes, 'codes')
-    M, C = ck.codes.shape
+    _on_gpu(ck)
+    M, C = ck.shape
     _channels(C, scale=scale, shift=shift)
     _check_bits(bits, M, C)
-    _same_device(ck.codes.device, scale=scale, shift=shift, bits=bits)
-    x = torch.empty((M, C), dtype=torch.float32, device=ck.codes.device)
+    _same_device(ck.device, scale=scale, shift=shift, bits=bits)
+    x = torch.empty((M, C), dtype=torch.float32, device=ck.device)
     lib = _lib.load()
     with _lib.on_device(x.device) as st:
-        _lib.check(lib.hmf_act8_restore_activation(ck.codes.data_ptr(), ck.exps.data_ptr(), None if bits is None else bits.data_ptr(), scale.data_ptr(),
+        _lib.check(lib.hmf_act8_restore_activation(ck.codes_ptr, ck.exps_ptr, None if bits is None else bits.data_ptr(), scale.data_ptr(),
                                                    shift.data_ptr(), x.data_ptr(), M, C, st), 'hmf_act8_restore_activation')
     return x
 
@@ -155,19 +176,19 @@ def bn_backward(g, ck, bits, mean, rstd, gamma, want_gz=False):
     _rows(g, 'g')
     M, C = g.shape
     _channels(C, mean=mean, rstd=rstd, gamma=gamma)
-    if tuple(ck.codes.shape) != (M, C):
-        raise ValueError('humaniflow_amd: the checkpoint holds %s rows, the gradient is %s' % (tuple(ck.codes.shape), (M, C)))
+    if ck.shape != g.shape:
+        raise ValueError('humaniflow_amd: the checkpoint holds %s rows, the gradient is %s' % (tuple(ck.shape), (M, C)))
     _check_bits(bits, M, C)
     dev = g.device
-    _same_device(dev, checkpoint=ck.codes, bits=bits, mean=mean, rstd=rstd, gamma=gamma)
+    _same_device(dev, checkpoint=ck, bits=bits, mean=mean, rstd=rstd, gamma=gamma)
     gy = torch.empty_like(g)
     gz = torch.empty_like(g) if want_gz else None
-    gg, gb = torch.empty(2, C, dtype=torch.float32, device=dev).unbind(0)
+    gg, gb = torch.empty_like(gamma), torch.empty_like(gamma)
     lib = _lib.load()
     n = int(lib.hmf_bn_backward_act8_workspace_bytes(M, C))
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev) as st:
-        _lib.check(lib.hmf_bn_backward_act8(g.data_ptr(), ck.codes.data_ptr(), ck.exps.data_ptr(), None if bits is None else bits.data_ptr(), mean.data_ptr(),
+        _lib.check(lib.hmf_bn_backward_act8(g.data_ptr(), ck.codes_ptr, ck.exps_ptr, None if bits is None else bits.data_ptr(), mean.data_ptr(),
                                             rstd.data_ptr(), gamma.data_ptr(), gy.data_ptr(), None if gz is None else gz.data_ptr(), gg.data_ptr(), gb.data_ptr(),
                                             M, C, ws.data_ptr(), n, st), 'hmf_bn_backward_act8')
     return gy, gz, gg, gb

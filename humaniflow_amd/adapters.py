@@ -18,52 +18,57 @@ from . import _lib, act8
 MAX_RANK = 64
 
 
+_TYPES = (torch.float32, torch.bfloat16)
+
+
 def _check(x, weight, bias, A, B, scale, ids):
-    """Shapes, types and devices -> (M, K, N, r, L, ids as int32)."""
-    dt = weight.dtype
-    if dt not in (torch.float32, torch.bfloat16):
+    """Shapes, types and devices (x: a tensor or an Act8) -> (M, K, N, r, L, ids as int32)."""
+    dt, ws, xs, As, Bs = weight.dtype, weight.shape, x.shape, A.shape, B.shape
+    if dt not in _TYPES:
         raise ValueError('humaniflow_amd: adapted_linear is built for float32 and bfloat16, got %s' % dt)
-    if weight.dim() != 2 or A.dim() != 3 or B.dim() != 3 or len(x.shape) != 2:
-        raise ValueError('humaniflow_amd: adapted_linear takes x (M, K), weight (N, K), A (L, r, K), B (L, N, r); got %s, %s, %s, %s'
-                         % (tuple(x.shape), tuple(weight.shape), tuple(A.shape), tuple(B.shape)))
-    M, K = x.shape
-    N = weight.shape[0]
-    L, r = A.shape[:2]
-    if weight.shape[1] != K or A.shape[2] != K or B.shape != (L, N, r) or L < 1 or r < 1 or K < 1 or N < 1:
-        raise ValueError('humaniflow_amd: adapted_linear: x %s, weight %s, A %s, B %s do not fit' % (tuple(x.shape), tuple(weight.shape), tuple(A.shape), tuple(B.shape)))
+    if len(ws) != 2 or len(As) != 3 or len(Bs) != 3 or len(xs) != 2:
+        raise ValueError('humaniflow_amd: adapted_linear takes x (M, K), weight (N, K), A (L, r, K), B (L, N, r); got %s, %s, %s, %s' % (tuple(xs), tuple(ws), tuple(As), tuple(Bs)))
+    M, K = xs
+    N, L, r = ws[0], As[0], As[1]
+    if ws[1] != K or As[2] != K or Bs != (L, N, r) or L < 1 or r < 1 or K < 1 or N < 1:
+        raise ValueError('humaniflow_amd: adapted_linear: x %s, weight %s, A %s, B %s do not fit' % (tuple(xs), tuple(ws), tuple(As), tuple(Bs)))
     if r > MAX_RANK:
         raise ValueError('humaniflow_amd: adapters of rank %d: built up to %d' % (r, MAX_RANK))
-    if A.dtype != dt or B.dtype != dt or (bias is not None and (bias.dtype != dt or tuple(bias.shape) != (N,))):
+    if A.dtype != dt or B.dtype != dt or (bias is not None and (bias.dtype != dt or bias.shape != (N,))):
         raise ValueError('humaniflow_amd: adapted_linear: bias (%d), A and B must have the weight\'s type %s' % (N, dt))
-    if scale.dtype != torch.float32 or tuple(scale.shape) != (L,):
+    if scale.dtype != torch.float32 or scale.shape != (L,):
         raise ValueError('humaniflow_amd: `scale` must be float32 (%d), got %s %s' % (L, scale.dtype, tuple(scale.shape)))
-    if ids.dtype not in (torch.int32, torch.int64) or tuple(ids.shape) != (M,):
+    if ids.shape != (M,) or ids.dtype not in (torch.int32, torch.int64):
         raise ValueError('humaniflow_amd: `ids` must be int32 or int64 (%d), got %s %s' % (M, ids.dtype, tuple(ids.shape)))
-    _lib.require_cuda(weight, 'weight')
+    if not weight.is_cuda:
+        _lib.require_cuda(weight, 'weight')
     dev = weight.device
-    for name, t in (('x', x), ('bias', bias), ('A', A), ('B', B), ('scale', scale), ('ids', ids)):
-        if t is not None and t.device != dev:
-            raise ValueError('humaniflow_amd: `%s` is on %s, the weight on %s' % (name, t.device, dev))
+    if x.device != dev or A.device != dev or B.device != dev or scale.device != dev or ids.device != dev or (bias is not None and bias.device != dev):
+        for name, t in (('x', x), ('bias', bias), ('A', A), ('B', B), ('scale', scale), ('ids', ids)):
+            if t is not None and t.device != dev:
+                raise ValueError('humaniflow_amd: `%s` is on %s, the weight on %s' % (name, t.device, dev))
     if ids.dtype == torch.int64:
         ids = ids.clamp(-1, 0x7fffffff).to(torch.int32)                  # what does not fit 32 bits stays out of range
-    return M, K, N, r, L, ids.contiguous()
+    return M, K, N, r, L, ids if ids.is_contiguous() else ids.contiguous()
 
 
 def _dense(t):
-    return None if t is None else t.detach().contiguous()
+    """t, or a contiguous copy of it (only its memory is used: no graph)."""
+    return t if t is None or t.is_contiguous() else t.detach().contiguous()
 
 
 def _rows(x):
     """x with consecutive columns (rows may have a pitch) and that pitch."""
-    x = x.detach()
     M, K = x.shape
+    if x.is_contiguous():
+        return x, K
     if (K > 1 and x.stride(1) != 1) or (M > 1 and x.stride(0) < K):
-        x = x.contiguous()
+        return x.detach().contiguous(), K
     return x, x.stride(0) if M > 1 else K
 
 
-def adapted_linear_forward(x, weight, bias, A, B, scale, ids):
-    """(y (M, N), t (M, r) float32): t = s_l A_l x is what the backward pass takes."""
+def adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t=True):
+    """(y (M, N), t (M, r) float32): t = s_l A_l x is what the backward pass takes (None without need_t)."""
     M, K, N, r, L, ids = _check(x, weight, bias, A, B, scale, ids)
     if x.dtype != weight.dtype:
         raise ValueError('humaniflow_amd: adapted_linear: x is %s, the weight %s' % (x.dtype, weight.dtype))
@@ -71,27 +76,28 @@ def adapted_linear_forward(x, weight, bias, A, B, scale, ids):
     weight, bias, A, B, scale = _dense(weight), _dense(bias), _dense(A), _dense(B), _dense(scale)
     dev = weight.device
     y = torch.empty((M, N), dtype=weight.dtype, device=dev)
-    t = torch.empty((M, r), dtype=torch.float32, device=dev)
+    t = torch.empty((M, r), dtype=torch.float32, device=dev) if need_t else None
     lib = _lib.load()
-    n = lib.hmf_adapted_linear_workspace_bytes(M, K, N, r, L, int(weight.dtype == torch.bfloat16))
+    bf16 = int(weight.dtype == torch.bfloat16)
+    n = lib.hmf_adapted_linear_workspace_bytes(M, K, N, r, L, bf16)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev) as st:
         _lib.check(lib.hmf_adapted_linear(x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(),
-                                          ids.data_ptr(), M, K, N, r, L, int(weight.dtype == torch.bfloat16), y.data_ptr(), t.data_ptr(), ws.data_ptr(), n, st),
+                                          ids.data_ptr(), M, K, N, r, L, bf16, y.data_ptr(), None if t is None else t.data_ptr(), ws.data_ptr(), n, st),
                    'hmf_adapted_linear')
     return y, t
 
 
 def adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=True):
     """(dL/dx or None, dL/dA, dL/dB) from dy = dL/dy; x: the forward's input or its 8-bit checkpoint; t: what the forward returned."""
-    kept = x.codes if isinstance(x, act8.Act8) else x
-    M, K, N, r, L, ids = _check(kept, weight, None, A, B, scale, ids)
+    kept8 = isinstance(x, act8.Act8)
+    M, K, N, r, L, ids = _check(x, weight, None, A, B, scale, ids)
     dt, dev = weight.dtype, weight.device
-    if not isinstance(x, act8.Act8) and x.dtype != dt:
+    if not kept8 and x.dtype != dt:
         raise ValueError('humaniflow_amd: adapted_linear: x is %s, the weight %s' % (x.dtype, dt))
-    if dy.dtype != dt or tuple(dy.shape) != (M, N) or dy.device != dev:
+    if dy.dtype != dt or dy.shape != (M, N) or dy.device != dev:
         raise ValueError('humaniflow_amd: `dy` must be %s (%d, %d) on %s, got %s %s on %s' % (dt, M, N, dev, dy.dtype, tuple(dy.shape), dy.device))
-    if t.dtype != torch.float32 or tuple(t.shape) != (M, r) or t.device != dev:
+    if t.dtype != torch.float32 or t.shape != (M, r) or t.device != dev:
         raise ValueError('humaniflow_amd: `t` must be float32 (%d, %d) on %s, got %s %s on %s' % (M, r, dev, t.dtype, tuple(t.shape), t.device))
     dy = _dense(dy)
     if dy.data_ptr() % 16:
@@ -99,11 +105,11 @@ def adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=True):
     t, weight, A, B, scale = _dense(t), _dense(weight), _dense(A), _dense(B), _dense(scale)
     if M == 0:
         return (torch.empty((0, K), dtype=dt, device=dev) if need_dx else None), torch.zeros_like(A), torch.zeros_like(B)
-    if isinstance(x, act8.Act8):
-        xp, ldx, exps = x.codes, K, x.exps
+    if kept8:
+        xp, ldx, exps = x.codes_ptr, K, x.exps_ptr
     else:
-        xp, ldx = _rows(x)
-        exps = None
+        x, ldx = _rows(x)
+        xp, exps = x.data_ptr(), None
     dx = torch.empty((M, K), dtype=dt, device=dev) if need_dx else None
     dA, dB = torch.empty_like(A), torch.empty_like(B)
     lib = _lib.load()
@@ -111,7 +117,7 @@ def adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=True):
     n = lib.hmf_adapted_linear_backward_workspace_bytes(M, K, N, r, L, bf16)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev) as st:
-        _lib.check(lib.hmf_adapted_linear_backward(dy.data_ptr(), xp.data_ptr(), ldx, None if exps is None else exps.data_ptr(), t.data_ptr(), weight.data_ptr(),
+        _lib.check(lib.hmf_adapted_linear_backward(dy.data_ptr(), xp, ldx, exps, t.data_ptr(), weight.data_ptr(),
                                                    A.data_ptr(), B.data_ptr(), scale.data_ptr(), ids.data_ptr(), M, K, N, r, L, bf16,
                                                    None if dx is None else dx.data_ptr(), dA.data_ptr(), dB.data_ptr(), ws.data_ptr(), n, st),
                    'hmf_adapted_linear_backward')
@@ -122,20 +128,16 @@ class _AdaptedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, A, B, scale, ids, checkpoint):
         y, t = adapted_linear_forward(x, weight, bias, A, B, scale, ids)
-        x = x.detach()
-        if checkpoint == 'int8':                                         # x itself is not kept
-            ck = act8.pack(x)
-            ctx.save_for_backward(ck.codes, ck.exps, t, weight, A, B, scale, ids)
-        else:
-            ctx.save_for_backward(x, None, t, weight, A, B, scale, ids)
+        ctx.ck = act8.pack(x) if checkpoint == 'int8' else None            # then x itself is not kept
+        ctx.save_for_backward(x if ctx.ck is None else None, t, weight, A, B, scale, ids)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, exps, t, weight, A, B, scale, ids = ctx.saved_tensors
-        if exps is not None:
-            x = act8.Act8(x, exps)
+        x, t, weight, A, B, scale, ids = ctx.saved_tensors
+        if ctx.ck is not None:
+            x = ctx.ck
         dx, dA, dB = adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=ctx.needs_input_grad[0])
         return dx, None, None, dA, dB, None, None, None
 
@@ -150,7 +152,7 @@ def adapted_linear(x, weight, bias, A, B, scale, ids, checkpoint=None):
             raise RuntimeError('humaniflow_amd: adapters are fitted beside a fixed projection: call requires_grad_(False) on its weight and bias, and on scale')
         if x.requires_grad or A.requires_grad or B.requires_grad:
             return _AdaptedLinear.apply(x, weight, bias, A, B, scale, ids, checkpoint)
-    return adapted_linear_forward(x, weight, bias, A, B, scale, ids)[0]
+    return adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t=False)[0]
 
 
 class LowRankAdapters(nn.Module):

@@ -14,6 +14,7 @@
 // bytes of a row) x a quarter of the rows (row 4 i + q), so a tile is 8 independent 16-byte loads per lane and the block maximum needs two shuffles per
 // channel; with the 32 rows of a block in one lane (no shuffle) the tensor of the last layer (4,608 x 512) is 288 waves on 1,024 SIMDs.
 #include <algorithm>
+#include <type_traits>
 #include "hmf_common.h"
 
 namespace hmf {
@@ -40,6 +41,20 @@ __device__ __forceinline__ float value_of(unsigned int word, int k, float step) 
     const int c = (int)(signed char)(word >> (8 * k));
     return c == -128 ? __uint_as_float(0x7fc00000u) : (float)c * step;
 }
+// a word of codes without the marker -128 (values_of's fast side): plain conversions
+__device__ __forceinline__ bool has_marker(unsigned int word) {
+    const unsigned int x = word ^ 0x80808080u;
+    return ((x - 0x01010101u) & ~x & 0x80808080u) != 0u;
+}
+template <bool MARKED> __device__ __forceinline__ float value_minus(unsigned int word, int k, float step, float sub) {
+    const int c = (int)(signed char)(word >> (8 * k));
+    const float v = fmaf((float)c, step, -sub);                            // the product is exact: one rounding
+    return MARKED && c == -128 ? __uint_as_float(0x7fc00000u) : v;
+}
+// v where bit b (a constant after unrolling) of the word is set, else 0: two integer operations
+__device__ __forceinline__ float where_bit(unsigned int word, int b, float v) {
+    return __uint_as_float(__float_as_uint(v) & (unsigned)__builtin_amdgcn_sbfe((int)word, b, 1));
+}
 __device__ __forceinline__ unsigned int max_over_quarters(unsigned int m) {
     m = max(m, (unsigned)__shfl_xor((int)m, 16));
     return max(m, (unsigned)__shfl_xor((int)m, 32));
@@ -50,6 +65,14 @@ __device__ __forceinline__ unsigned short f32_to_bf16(float f) {
     const unsigned int u = __float_as_uint(f);
     if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)((u >> 16) | 0x40u);
     return (unsigned short)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+
+// NT: past the caches.  A map of more than half the Infinity Cache (256 MB) is gone from it before its reader comes, and only pushes out what the next kernels
+// read: the backward of 294,912 x 256 takes 247 us with, 269 us without; a small map's reader finds it there.  (The forward's map: 202 us without, 207 us with.)
+constexpr long long kStreamBytes = 128ll << 20;
+template <bool NT> __device__ __forceinline__ void store4(float* p, f32x4 v) {
+    if (NT) __builtin_nontemporal_store(v, (f32x4*)p);
+    else *(f32x4*)p = v;
 }
 
 // lane's V consecutive columns of one row: 16 bytes
@@ -351,20 +374,27 @@ __global__ __launch_bounds__(256) void k_bn8_reduce(const float* __restrict__ g,
         const unsigned int e = *(const unsigned int*)(exps + (long long)t * C + c);
         uint4 b = make_uint4(~0u, ~0u, ~0u, ~0u);
         if (bits) b = *(const uint4*)(bits + (long long)t * C + c);
-        const unsigned int on[4] = {b.x, b.y, b.z, b.w};
+        const unsigned int on[4] = {b.x >> q, b.y >> q, b.z >> q, b.w >> q};
+        auto add = [&](auto MARKED) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float st = step_of((int)((e >> (8 * k)) & 0xffu));
-            float s = 0.f, sx = 0.f;
+            for (int k = 0; k < 4; ++k) {
+                const float st = step_of((int)((e >> (8 * k)) & 0xffu));
+                float s = 0.f, sx = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float gz = ((on[k] >> (4 * i + q)) & 1u) ? gv[i][k] : 0.f;
-                s += gz;
-                sx = fmaf(gz, (value_of(w[i], k, st) - mu[k]) * rs[k], sx);
+                for (int i = 0; i < 8; ++i) {
+                    const float gz = where_bit(on[k], 4 * i, gv[i][k]);
+                    s += gz;
+                    sx = fmaf(gz, value_minus<decltype(MARKED)::value>(w[i], k, st, mu[k]), sx);
+                }
+                S[k] += (double)s;
+                SX[k] += (double)(sx * rs[k]);
             }
-            S[k] += (double)s;
-            SX[k] += (double)sx;
-        }
+        };
+        bool marked = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) marked |= has_marker(w[i]);
+        if (__any(marked)) add(std::true_type{});
+        else add(std::false_type{});
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -387,24 +417,39 @@ __global__ __launch_bounds__(256) void k_bn8_reduce(const float* __restrict__ g,
     }
 }
 
-// coef[0][c] = gamma rstd, coef[1][c] = sg / M, coef[2][c] = sgx / M; 16 lanes per channel walk the partial sums
+// coef[0][c] = gamma rstd, coef[1][c] = sg / M, coef[2][c] = sgx / M; 64 lanes per channel walk the partial sums, four channels a work-group (16 lanes: 576 partial sums
+// of 256 channels took 14 us)
 __global__ __launch_bounds__(256) void k_bn8_finalize(const double* __restrict__ part, int nparts, int M, int C, const float* __restrict__ gamma,
                                                       const float* __restrict__ rstd, float* __restrict__ g_gamma, float* __restrict__ g_beta,
                                                       float* __restrict__ coef) {
-    __shared__ double red[2][16][17];
-    const int cl = threadIdx.x & 15, j = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+    __shared__ double red[2][64][5];
+    const int cl = threadIdx.x & 3, j = threadIdx.x >> 2, c = blockIdx.x * 4 + cl;
     double s = 0.0, sx = 0.0;
-    for (int p = j; p < nparts; p += 16) {
-        s += part[(long long)p * 2 * C + c];
-        sx += part[((long long)p * 2 + 1) * C + c];
+    for (int p0 = j; p0 < nparts; p0 += 64 * 4) {
+        double v[4], w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const long long p = min(p0 + 64 * k, nparts - 1);
+            v[k] = part[p * 2 * C + c];
+            w[k] = part[(p * 2 + 1) * C + c];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (p0 + 64 * k < nparts) { s += v[k]; sx += w[k]; }
     }
     red[0][j][cl] = s;
     red[1][j][cl] = sx;
     __syncthreads();
-    if (threadIdx.x < 16) {
-        double a = 0.0, b = 0.0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) { a += red[0][k][cl]; b += red[1][k][cl]; }
+    for (int d = 32; d >= 1; d >>= 1) {
+        if (j < d) {
+            red[0][j][cl] += red[0][j + d][cl];
+            red[1][j][cl] += red[1][j + d][cl];
+        }
+        __syncthreads();
+    }
+    if (j == 0) {
+        const double a = red[0][0][cl], b = red[1][0][cl];
         g_beta[c] = (float)a;
         g_gamma[c] = (float)b;
         coef[c] = gamma[c] * rstd[c];
@@ -413,45 +458,58 @@ __global__ __launch_bounds__(256) void k_bn8_finalize(const double* __restrict__
     }
 }
 
-template <bool GZ>
+template <bool GZ, bool NT>
 __global__ __launch_bounds__(256) void k_bn8_apply(const float* __restrict__ g, const unsigned char* __restrict__ codes, const unsigned char* __restrict__ exps,
                                                    const unsigned int* __restrict__ bits, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                    const float* __restrict__ coef, float* __restrict__ gy, float* __restrict__ gz_out, int M, int C, int ct,
                                                    long long tiles) {
-    const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (tile >= tiles) return;
+    // last tile first: the reduction ended there, and what it read last is still in the Infinity Cache
+    const long long tile = tiles - 1 - ((long long)blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (tile < 0) return;
     const int lane = threadIdx.x & 63, q = lane >> 4;
     const int t = (int)(tile / ct), c = (int)(tile - (long long)t * ct) * 64 + (lane & 15) * 4;
     const int m0 = t * 32 + q;
     f32x4 gv[8];
     unsigned int w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
+        w[i] = 0u;
         if (m0 + 4 * i < M) {
             const long long o = (long long)(m0 + 4 * i) * C + c;
             gv[i] = *(const f32x4*)(g + o);
             w[i] = *(const unsigned int*)(codes + o);
         }
+    }
     const unsigned int e = *(const unsigned int*)(exps + (long long)t * C + c);
     uint4 b = make_uint4(~0u, ~0u, ~0u, ~0u);
     if (bits) b = *(const uint4*)(bits + (long long)t * C + c);
-    const unsigned int on[4] = {b.x, b.y, b.z, b.w};
+    const unsigned int on[4] = {b.x >> q, b.y >> q, b.z >> q, b.w >> q};
     const f32x4 mu = *(const f32x4*)(mean + c), rs = *(const f32x4*)(rstd + c);
     const f32x4 ca = *(const f32x4*)(coef + c), cs = *(const f32x4*)(coef + C + c), cx = *(const f32x4*)(coef + 2 * C + c);
+    float st[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (m0 + 4 * i < M) {
-            f32x4 z, o;
+    for (int k = 0; k < 4; ++k) st[k] = step_of((int)((e >> (8 * k)) & 0xffu));
+    auto write = [&](auto MARKED) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float xh = (value_of(w[i], k, step_of((int)((e >> (8 * k)) & 0xffu))) - mu[k]) * rs[k];
-                z[k] = ((on[k] >> (4 * i + q)) & 1u) ? gv[i][k] : 0.f;
-                o[k] = ca[k] * ((z[k] - cs[k]) - xh * cx[k]);
+        for (int i = 0; i < 8; ++i)
+            if (m0 + 4 * i < M) {
+                f32x4 z, o;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float xh = value_minus<decltype(MARKED)::value>(w[i], k, st[k], mu[k]) * rs[k];
+                    z[k] = where_bit(on[k], 4 * i, gv[i][k]);
+                    o[k] = ca[k] * ((z[k] - cs[k]) - xh * cx[k]);
+                }
+                const long long at = (long long)(m0 + 4 * i) * C + c;
+                store4<NT>(gy + at, o);
+                if (GZ) store4<NT>(gz_out + at, z);
             }
-            const long long at = (long long)(m0 + 4 * i) * C + c;
-            *(f32x4*)(gy + at) = o;
-            if (GZ) *(f32x4*)(gz_out + at) = z;
-        }
+    };
+    bool marked = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) marked |= has_marker(w[i]);
+    if (__any(marked)) write(std::true_type{});
+    else write(std::false_type{});
 }
 
 // Tiles of 32 rows per work-group of the reduction: enough work-groups for the 256 CUs first, then up to 16 tiles (512 rows) each
@@ -582,12 +640,17 @@ int hmf_bn_backward_act8(const float* g, const signed char* codes, const unsigne
     const unsigned char* cd = (const unsigned char*)codes;
     hipLaunchKernelGGL(k_bn8_reduce, dim3(ct, parts), dim3(256), 0, st, g, cd, exps, bits, mean, rstd, M, C, per, part);
     HMF_LAUNCH_CHECK();
-    hipLaunchKernelGGL(k_bn8_finalize, dim3(C / 16), dim3(256), 0, st, part, parts, M, C, gamma, rstd, g_gamma, g_beta, coef);
+    hipLaunchKernelGGL(k_bn8_finalize, dim3(C / 4), dim3(256), 0, st, part, parts, M, C, gamma, rstd, g_gamma, g_beta, coef);
     HMF_LAUNCH_CHECK();
     const long long tiles = (long long)((M + 31) / 32) * ct;
     const dim3 grid((unsigned)((tiles + 3) / 4)), block(256);
-    if (gz) hipLaunchKernelGGL(k_bn8_apply<true>, grid, block, 0, st, g, cd, exps, bits, mean, rstd, coef, gy, gz, M, C, ct, tiles);
-    else hipLaunchKernelGGL(k_bn8_apply<false>, grid, block, 0, st, g, cd, exps, bits, mean, rstd, coef, gy, gz, M, C, ct, tiles);
+    const bool nt = (long long)M * C * 4 > kStreamBytes;
+#define HMF_BN8A(GZ, NT) hipLaunchKernelGGL((k_bn8_apply<GZ, NT>), grid, block, 0, st, g, cd, exps, bits, mean, rstd, coef, gy, gz, M, C, ct, tiles)
+    if (gz && nt) HMF_BN8A(true, true);
+    else if (gz) HMF_BN8A(true, false);
+    else if (nt) HMF_BN8A(false, true);
+    else HMF_BN8A(false, false);
+#undef HMF_BN8A
     HMF_LAUNCH_CHECK();
     return HMF_OK;
 }

@@ -200,24 +200,47 @@ __global__ __launch_bounds__(256) void k_ad_few(const AdArgs<T> a, int tiles_o, 
     base_tile<T, true, VEC>(a, a.x, a.ldx, a.N, a.K, ot, rest % a.ksplit, rest / a.ksplit, red);
 }
 
+// sum of n values `stride` apart, eight loads in flight (a plain loop waits for every one: 16 splits took 7 us)
+__device__ __forceinline__ float sum_strided(const float* p, int n, long long stride) {
+    float v = 0.f;
+    for (int k0 = 0; k0 < n; k0 += 8) {
+        float q[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[k] = p[(long long)min(k0 + k, n - 1) * stride];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += k0 + k < n ? q[k] : 0.f;
+    }
+    return v;
+}
+// sum_j low[j] w[j * stride], eight loads of each in flight
+template <typename T> __device__ __forceinline__ float dot_strided(const float* low, const T* w, int r, long long stride) {
+    float v = 0.f;
+    for (int j0 = 0; j0 < r; j0 += 8) {
+        float a[8];
+        T b[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            a[k] = low[min(j0 + k, r - 1)];
+            b[k] = w[(long long)min(j0 + k, r - 1) * stride];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (j0 + k < r) v = fmaf(a[k], up(b[k]), v);
+    }
+    return v;
+}
+
 // y = partial sums + bias + B_l t
 template <typename T>
-__global__ __launch_bounds__(256) void k_ad_join(const AdArgs<T> a) {
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x, n_all = (long long)a.M * a.N;
+__global__ __launch_bounds__(64) void k_ad_join(const AdArgs<T> a) {
+    const long long e = (long long)blockIdx.x * 64 + threadIdx.x, n_all = (long long)a.M * a.N;
     if (e >= n_all) return;
     const int m = (int)(e / a.N), n = (int)(e - (long long)m * a.N);
-    float v = a.partial[e];
-    for (int k = 1; k < a.ksplit; ++k) v += a.partial[(long long)k * n_all + e];
-    if (a.bias) v += up(a.bias[n]);
     const int l = a.ids[m];
+    float v = sum_strided(a.partial + e, a.ksplit, n_all);
+    if (a.bias) v += up(a.bias[n]);
     if (l >= a.L) v = nan32();
-    else if (l >= 0) {
-        const T* br = a.b + ((long long)l * a.N + n) * a.r;
-        const float* tr = a.t + (long long)m * a.r;
-        float d = 0.f;
-        for (int j = 0; j < a.r; ++j) d = fmaf(tr[j], up(br[j]), d);
-        v += d;
-    }
+    else if (l >= 0) v += dot_strided(a.t + (long long)m * a.r, a.b + ((long long)l * a.N + n) * a.r, a.r, 1);
     down(a.y + e, v);
 }
 
@@ -312,7 +335,7 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
         f32x4 acc[8];
 #pragma unroll
         for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        constexpr int U = 4;
+        constexpr int U = 8;
         for (int rr = r0; rr < r1; rr += 4 * U) {
             Z8<T, ACT8> z[U];
             float pv[U];
@@ -442,17 +465,10 @@ __global__ __launch_bounds__(256) void k_ad_few_back2(const AdArgs<T> a, const A
         const long long e = (long long)id * 256 + threadIdx.x, n_all = (long long)a.M * a.K;
         if (e >= n_all) return;
         const int m = (int)(e / a.K), k = (int)(e - (long long)m * a.K);
-        float v = a.partial[e];
-        for (int s = 1; s < a.ksplit; ++s) v += a.partial[(long long)s * n_all + e];
         const int l = a.ids[m];
+        float v = sum_strided(a.partial + e, a.ksplit, n_all);
         if (l >= a.L) v = nan32();
-        else if (l >= 0) {
-            const T* ar = a.a + (long long)l * a.r * a.K + k;
-            const float* ur = a.u + (long long)m * a.r;
-            float d = 0.f;
-            for (int j = 0; j < a.r; ++j) d = fmaf(ur[j], up(ar[(long long)j * a.K]), d);
-            v += d;
-        }
+        else if (l >= 0) v += dot_strided(a.u + (long long)m * a.r, a.a + (long long)l * a.r * a.K + k, a.r, a.K);
         down(a.dx + e, v);
         return;
     }
@@ -722,21 +738,24 @@ template <typename T> struct AdGemm {
     int per;                                // chunks of a split
 };
 
-// BT x BT tile, 4 waves of (BT / 2) x (BT / 2); a ring of 4 LDS stages of one chunk (128 bytes of every row of both operands) filled by LDS-DMA three chunks
-// ahead: with one chunk ahead through registers the 128-tile took 2.2 us a chunk, the latency of its loads.  The 16-byte slot c of row r lies at slot
-// c ^ ((r >> 1) & 7) (the DMA writes in lane order, so the source address is permuted): a fragment read hits every bank once.
+// BT x BT tile, 4 waves of (BT / 2) x (BT / 2); a ring of 4 LDS stages of one chunk (RB bytes of every row of both operands) filled by LDS-DMA three chunks ahead:
+// with one chunk ahead through registers a chunk of the 128-tile took 2.2 us, the latency of its loads; so 0.46 us (32 KB read from and 16 KB written to LDS
+// for 512 cycles of MFMA).  The 16-byte slot c of row r lies at slot c ^ swizzle(r) (the DMA writes in lane order, so the source address is permuted): a
+// fragment read hits every bank once.  RB = 128 (whole lines, one work-group per CU at BT = 128) where a CU has one tile; RB = 64 (half the LDS: two work-groups
+// per CU, one's start and end under the other's products) where it has more (4,096 rows, 1,024 -> 2,048, bfloat16: 55 -> 44 us).
 // After the shared weight's chunks come the adapters': 16-byte piece P of a row belongs to the tile's adapter list[P / pp] and holds E of its ranks (bfloat16: the
 // high halves of all ranks, then the low ones).  The rows of other adapters hold zeros there,
 // and a zero times an infinity or a NaN of a weight would reach them: such weights are staged as zeros and added to their own rows at the end.
-template <typename T, int BT>
+template <typename T, int BT, int RB>
 __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
     typedef Mma<T> X;
     typedef typename X::frag frag;
-    constexpr int BK = X::BK, E = X::E, S = 4;
-    constexpr int ND = BT / 32;                                             // DMA requests of a wave, operand and chunk (8 rows each)
+    constexpr int E = X::E, S = 4, PR = RB / 16, G = RB / 32;               // 16-byte pieces and MFMA groups of a row's chunk
+    constexpr int ND = BT * RB / 4096;                                      // DMA requests of a wave, operand and chunk (1 KB each)
     constexpr int NT = BT / 64;                                             // MFMA tiles of a wave, each way
-    constexpr int NS = BT * 8 / 256;                                        // 16-byte pieces of a thread, operand and chunk
-    constexpr int OP = BT * 128, STAGE = 2 * OP;                            // bytes
+    constexpr int NS = BT * PR / 256;                                       // pieces of a thread, operand and chunk
+    constexpr int OP = BT * RB, STAGE = 2 * OP;                             // bytes
+    auto swizzle = [](int row) { return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
     __shared__ __attribute__((aligned(16))) char smem[S * STAGE + (3 * BT + 4) * 4];      // one object: a second one makes hipcc wait for the DMA before every read
     int* rowid = (int*)(smem + S * STAGE);
     int *slot = rowid + BT, *list = slot + BT, *nlist = list + BT, *odd = nlist + 2;
@@ -769,25 +788,25 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
     }
     __syncthreads();
     // chunks of this split; 16-byte pieces of an adapter's ranks, of an adapter, of all (the first split's), and their chunks
-    const int cfirst = blockIdx.y * a.per, kc = min(a.per, a.C / BK - cfirst);
-    const int pr = (a.r + E - 1) / E, pp = pr * X::HL, ext = blockIdx.y == 0 ? nad * pp : 0, ne = (ext + 7) / 8;
+    const int cfirst = blockIdx.y * a.per, kc = min(a.per, a.C * (int)sizeof(T) / RB - cfirst);
+    const int pr = (a.r + E - 1) / E, pp = pr * X::HL, ext = blockIdx.y == 0 ? nad * pp : 0, ne = (ext + PR - 1) / PR;
 
-    // DMA sources: request d of wave w brings rows 8 (w ND + d) .. + 7; rows that are not there read a valid one, whose results are not stored
+    // DMA sources: request d of wave w brings rows 64 / PR (w ND + d) ..; rows that are not there read a valid one, whose results are not stored
     const char *gw[ND], *gx[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-        const int row = (wave * ND + d) * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
-        gw[d] = (const char*)(a.w + (long long)min(o0 + row, a.O - 1) * a.ldw) + 16 * c + (long long)cfirst * 128;
+        const int row = (wave * ND + d) * (64 / PR) + lane / PR, c = (lane % PR) ^ swizzle(row);
+        gw[d] = (const char*)(a.w + (long long)min(o0 + row, a.O - 1) * a.ldw) + 16 * c + (long long)cfirst * RB;
         const int m = rowid[row];
-        gx[d] = (const char*)(a.in + (long long)(m < 0 ? -1 - m : m) * a.ldin) + 16 * c + (long long)cfirst * 128;
+        gx[d] = (const char*)(a.in + (long long)(m < 0 ? -1 - m : m) * a.ldin) + 16 * c + (long long)cfirst * RB;
     }
     auto issue = [&](int c, int lo, int hi) {
         char* st = smem + (c & (S - 1)) * STAGE + wave * ND * 1024;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             if (d < lo || d >= hi) continue;
-            ad_dma16(gw[d] + (long long)c * 128, st + d * 1024);
-            ad_dma16(gx[d] + (long long)c * 128, st + OP + d * 1024);
+            ad_dma16(gw[d] + (long long)c * RB, st + d * 1024);
+            ad_dma16(gx[d] + (long long)c * RB, st + OP + d * 1024);
         }
     };
     // the adapters' chunks go through registers: raw values first, so that the first of them are loaded under the main loop.  A thread's pieces lie in the same column.
@@ -796,13 +815,13 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
     const bool vec_v = a.vj == 1 && a.r % E == 0 && ((uintptr_t)a.v & 15) == 0;
     int elo = 0;
     auto fetch = [&](int c) {
-        const int P = c * 8 + (tid & 7), ad = P / pp, rem = P - ad * pp, j0 = (rem >= pr ? rem - pr : rem) * E;
+        const int P = c * PR + tid % PR, ad = P / pp, rem = P - ad * pp, j0 = (rem >= pr ? rem - pr : rem) * E;
         elo = rem >= pr;
         const bool live = P < ext;
         const T* vb = a.v + (live ? (long long)list[ad] : 0ll) * a.vl + j0 * a.vj;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const int row = (tid + 256 * s) >> 3, o = o0 + row;
+            const int row = (tid + 256 * s) / PR, o = o0 + row;
             const bool mine = live && slot[row] == ad;
             const float* pl = a.low + (long long)(mine ? rowid[row] : 0) * a.r + j0;
 #pragma unroll
@@ -820,7 +839,7 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
     auto stash = [&](int st) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const int e = tid + 256 * s, row = e >> 3, at = row * 128 + (((e & 7) ^ ((row >> 1) & 7)) * 16);
+            const int e = tid + 256 * s, row = e / PR, at = row * RB + ((e % PR) ^ swizzle(row)) * 16;
             frag zw = ew[s], zx;
             bool ok = true;
 #pragma unroll
@@ -846,16 +865,16 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[t][v][e] = 0.f;
     const int wo = (wave & 1) * (BT / 2), wm = (wave >> 1) * (BT / 2);
-    const char *pw = smem + (wo + i) * 128, *px = smem + OP + (wm + i) * 128;
-    int go[4];
+    const char *pw = smem + (wo + i) * RB, *px = smem + OP + (wm + i) * RB;
+    int go[G];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) go[g] = ((2 * g + q) ^ ((i >> 1) & 7)) * 16;
+    for (int g = 0; g < G; ++g) go[g] = ((2 * g + q) ^ swizzle(i)) * 16;
     frag fw[2][NT], fx[2][NT];
     auto frags = [&](int st, int g) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            fw[g & 1][t] = *(const frag*)(pw + st * STAGE + go[g] + t * 4096);
-            fx[g & 1][t] = *(const frag*)(px + st * STAGE + go[g] + t * 4096);
+            fw[g & 1][t] = *(const frag*)(pw + st * STAGE + go[g] + t * 32 * RB);
+            fx[g & 1][t] = *(const frag*)(px + st * STAGE + go[g] + t * 32 * RB);
         }
     };
     auto mma = [&](int g) {
@@ -878,9 +897,9 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
         asm volatile("" ::: "memory");
         const int st = c & (S - 1);
         constexpr int nm = NT * NT * (sizeof(T) == 4 ? 4 : 1);
-        auto group = [&](auto G) {
-            constexpr int g = decltype(G)::value;
-            if (g < 3) frags(st, g + 1);
+        auto group = [&](auto index) {
+            constexpr int g = decltype(index)::value;
+            if (g + 1 < G) frags(st, g + 1);
             else if (more || c + 1 < kc) frags((c + 1) & (S - 1), 0);
             mma(g);
             if (more && g < ND) issue(c + S - 1, g, g + 1);                 // into the stage that everybody has read (chunk c - 1)
@@ -893,8 +912,10 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
         };
         group(std::integral_constant<int, 0>{});
         group(std::integral_constant<int, 1>{});
-        group(std::integral_constant<int, 2>{});
-        group(std::integral_constant<int, 3>{});
+        if constexpr (G == 4) {
+            group(std::integral_constant<int, 2>{});
+            group(std::integral_constant<int, 3>{});
+        }
     };
     if (kc >= S - 1) HMF_AD_VMCNT(2 * 2 * ND);                              // the first chunk
     else HMF_AD_VMCNT(0);
@@ -907,8 +928,8 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
     auto compute = [&](int st) {
         frags(st, 0);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            if (g < 3) frags(st, g + 1);
+        for (int g = 0; g < G; ++g) {
+            if (g + 1 < G) frags(st, g + 1);
             mma(g);
         }
     };
@@ -924,15 +945,8 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
     // BT / 2 outputs.
     const bool any_odd = *odd != 0;
     constexpr int H = BT / 2, PF = H + 4;                                   // outputs of a wave's rows, pitch in floats
-    static_assert(4 * H * PF * 4 <= S * STAGE, "the turned tiles lie in the ring");
-    float* tw = (float*)smem + wave * H * PF;
-#pragma unroll
-    for (int v = 0; v < NT; ++v)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e4 = 0; e4 < 4; ++e4)
-                *(f32x4*)(tw + (32 * v + i) * PF + 32 * t + 8 * e4 + 4 * q) = f32x4{acc[t][v][4 * e4], acc[t][v][4 * e4 + 1], acc[t][v][4 * e4 + 2], acc[t][v][4 * e4 + 3]};
+    static_assert(4 * 32 * PF * 4 <= S * STAGE, "the turned tiles lie in the ring");
+    float* tw = (float*)smem + wave * 32 * PF;
     constexpr int LPR = H / E, RPI = 64 / LPR;                              // lanes of a row, rows of an instruction
     const int oc = (lane % LPR) * E, o = o0 + wo + oc;
     const bool vec = a.O % E == 0 && ((uintptr_t)a.out & 15) == 0;
@@ -940,45 +954,53 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
 #pragma unroll
     for (int k = 0; k < E; ++k) bv[k] = (a.bias && !a.partial && o + k < a.O) ? up(a.bias[o + k]) : 0.f;
 #pragma unroll
-    for (int s = 0; s < H / RPI; ++s) {
-        const int row = s * RPI + lane / LPR, m = rowid[wm + row];
-        float z[E];
+    for (int v = 0; v < NT; ++v) {
 #pragma unroll
-        for (int k = 0; k < E; k += 4) {
-            const f32x4 u = *(const f32x4*)(tw + row * PF + oc + k);
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[k + e] = u[e] + bv[k + e];
-        }
-        if (m < 0 || o >= a.O) continue;
-        const int sl = slot[wm + row];
-        if (sl == -2 || any_odd) {
-            const int id = sl >= 0 ? list[sl] : -1;
+            for (int e4 = 0; e4 < 4; ++e4)
+                *(f32x4*)(tw + i * PF + 32 * t + 8 * e4 + 4 * q) = f32x4{acc[t][v][4 * e4], acc[t][v][4 * e4 + 1], acc[t][v][4 * e4 + 2], acc[t][v][4 * e4 + 3]};
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
-                if (sl == -2) z[k] = nan32();
-                else if (id >= 0 && o + k < a.O)
-                    for (int j = 0; j < a.r; ++j) {
-                        const T vv = a.v[id * a.vl + (o + k) * a.vo + j * a.vj];
-                        if (!finite(vv)) z[k] = fmaf(a.low[(long long)m * a.r + j], up(vv), z[k]);
-                    }
+        for (int s = 0; s < 32 / RPI; ++s) {
+            const int row = s * RPI + lane / LPR, at = wm + 32 * v + row, m = rowid[at];
+            float z[E];
+#pragma unroll
+            for (int k = 0; k < E; k += 4) {
+                const f32x4 u = *(const f32x4*)(tw + row * PF + oc + k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[k + e] = u[e] + bv[k + e];
             }
+            if (m < 0 || o >= a.O) continue;
+            const int sl = slot[at];
+            if (sl == -2 || any_odd) {
+                const int id = sl >= 0 ? list[sl] : -1;
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    if (sl == -2) z[k] = nan32();
+                    else if (id >= 0 && o + k < a.O)
+                        for (int j = 0; j < a.r; ++j) {
+                            const T vv = a.v[id * a.vl + (o + k) * a.vo + j * a.vj];
+                            if (!finite(vv)) z[k] = fmaf(a.low[(long long)m * a.r + j], up(vv), z[k]);
+                        }
+                }
+            }
+            if (a.partial) {
+                float* pp_ = a.partial + ((long long)blockIdx.y * a.M + m) * a.O + o;
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (o + k < a.O) pp_[k] = z[k];
+                continue;
+            }
+            T h[E] __attribute__((aligned(16)));
+#pragma unroll
+            for (int k = 0; k < E; ++k) down(h + k, z[k]);
+            T* po = a.out + (long long)m * a.O + o;
+            if (vec) *(uint4*)po = *(const uint4*)h;
+            else
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (o + k < a.O) po[k] = h[k];
         }
-        if (a.partial) {
-            float* pp_ = a.partial + ((long long)blockIdx.y * a.M + m) * a.O + o;
-#pragma unroll
-            for (int k = 0; k < E; ++k)
-                if (o + k < a.O) pp_[k] = z[k];
-            continue;
-        }
-        T h[E] __attribute__((aligned(16)));
-#pragma unroll
-        for (int k = 0; k < E; ++k) down(h + k, z[k]);
-        T* po = a.out + (long long)m * a.O + o;
-        if (vec) *(uint4*)po = *(const uint4*)h;
-        else
-#pragma unroll
-            for (int k = 0; k < E; ++k)
-                if (o + k < a.O) po[k] = h[k];
     }
 }
 
@@ -1009,32 +1031,29 @@ __global__ __launch_bounds__(256) void k_ad_grads(const AdGrad da, const AdGrad 
     else grad_piece<T, false>(db, r, rows, n, l, blockIdx.y, np == 1, cb - da.blocks, red);
 }
 
-// sums of the adapters that had several pieces, in the pieces' order; one work-group per (adapter, 256 elements of dA_l or dB_l)
+// sums of the adapters that had several pieces, in the pieces' order; a column of work-groups per adapter, gone at once where there is nothing to add
 template <typename T>
-__global__ __launch_bounds__(256) void k_ad_grad_join(const AdGrad da, const AdGrad db, const int* __restrict__ seg, int r, int L, int wa) {
-    const int l = blockIdx.y;
-    if (seg[l + 1] - seg[l] <= kFewRows) return;
-    int first = 0, np = 0;
-    {                                                                      // pieces in front of this adapter's
-        const int lane = threadIdx.x & 63;
-        for (int l0 = 0; l0 < l; l0 += 64) {
-            const int li = l0 + lane;
-            int v = li < l ? max(1, (seg[li + 1] - seg[li] + kFewRows - 1) / kFewRows) : 0;
+__global__ __launch_bounds__(256) void k_ad_grad_join(const AdGrad da, const AdGrad db, const int* __restrict__ seg, int r, int L) {
+    const int l = blockIdx.y, mine = seg[l + 1] - seg[l];
+    if (mine <= kFewRows) return;
+    const int lane = threadIdx.x & 63, np = (mine + kFewRows - 1) / kFewRows;
+    int first = 0;                                                         // pieces in front of this adapter's
+    for (int l0 = 0; l0 < l; l0 += 64) {
+        const int li = l0 + lane;
+        int v = li < l ? max(1, (seg[li + 1] - seg[li] + kFewRows - 1) / kFewRows) : 0;
 #pragma unroll
-            for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-            first += v;
-        }
-        np = (seg[l + 1] - seg[l] + kFewRows - 1) / kFewRows;
+        for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+        first += v;
     }
-    const bool is_a = (int)blockIdx.x < wa;
-    const AdGrad& g = is_a ? da : db;
-    const long long e = (long long)(is_a ? blockIdx.x : blockIdx.x - wa) * 256 + threadIdx.x, n = (long long)r * g.C;
-    if (e >= n) return;
-    float v = 0.f;
-    for (int p = 0; p < np; ++p) v += g.part[(long long)(first + p) * n + e];
-    const int j = (int)(e / g.C), c = (int)(e - (long long)j * g.C);
-    if (g.trans) down((T*)g.out + ((long long)l * g.C + c) * r + j, v);
-    else down((T*)g.out + ((long long)l * r + j) * g.C + c, v);
+    const long long na = (long long)r * da.C, n = na + (long long)r * db.C;
+    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
+        const AdGrad& g = at < na ? da : db;
+        const long long e = at < na ? at : at - na;
+        const float v = sum_strided(g.part + (long long)first * r * g.C + e, np, (long long)r * g.C);
+        const int j = (int)(e / g.C), c = (int)(e - (long long)j * g.C);
+        if (g.trans) down((T*)g.out + ((long long)l * g.C + c) * r + j, v);
+        else down((T*)g.out + ((long long)l * r + j) * g.C + c, v);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -1054,17 +1073,20 @@ static void few_split(int M, int O, int Cn, int* ksplit, int* kw) {
 }
 
 // Tiles of 128 where they fill three quarters of the CUs, else of 64; where those leave CUs idle too, the reduction is split until two work-groups go on each CU, but
-// not under 8 chunks (512 rows, 2,048 -> 1,024 in 32 bits, 128 tiles: 44 us unsplit).
-static void gemm_shape(int M, int O, int Cp, size_t z, int* bt, int* splits, int* per) {
-    *bt = (long long)blocks_of(M, 128) * blocks_of(O, 128) >= 192 ? 128 : 64;
-    const int kc = (int)(Cp * z / 128), tiles = blocks_of(M, *bt) * blocks_of(O, *bt);
-    const int want = tiles >= 256 ? 1 : std::max(1, std::min(kc / 8, 512 / tiles));
+// not under 8 chunks in 32 bits (512 rows, 2,048 -> 1,024, 128 tiles: 44 us unsplit, 28 us and 4 us for the sum in four) and 16 in bfloat16, whose chunk takes an
+// eighth of the matrix time (19 us unsplit, 17.5 + 4 us in four).
+static void gemm_shape(int M, int O, int Cp, size_t z, int* bt, int* rb, int* splits, int* per) {
+    const long long big = (long long)blocks_of(M, 128) * blocks_of(O, 128);
+    *bt = big >= 192 ? 128 : 64;
+    *rb = big > 256 && z == 2 ? 64 : 128;
+    const int kc = (int)(Cp * z / *rb), tiles = blocks_of(M, *bt) * blocks_of(O, *bt);
+    const int want = tiles >= 256 ? 1 : std::max(1, std::min(kc / (z == 4 ? 8 : 16), 512 / tiles));
     *per = blocks_of(kc, want);
     *splits = blocks_of(kc, *per);
 }
 static size_t gemm_partial(int M, int O, int Cp, size_t z) {
-    int bt, splits, per;
-    gemm_shape(M, O, Cp, z, &bt, &splits, &per);
+    int bt, rb, splits, per;
+    gemm_shape(M, O, Cp, z, &bt, &rb, &splits, &per);
     return splits > 1 ? (size_t)splits * M * O * 4 : 0;
 }
 // the many-row form's rows: whole chunks of 128 bytes, 16-byte aligned
@@ -1139,13 +1161,14 @@ template <typename T> static int prepare(const AdPrep& p, hipStream_t st) {
     return HMF_OK;
 }
 template <typename T> static int gemm(AdGemm<T>& m, void* partial, hipStream_t st) {
-    int bt, splits;
-    gemm_shape(m.M, m.O, m.C, sizeof(T), &bt, &splits, &m.per);
+    int bt, rb, splits;
+    gemm_shape(m.M, m.O, m.C, sizeof(T), &bt, &rb, &splits, &m.per);
     m.tiles_o = blocks_of(m.O, bt);
     m.partial = splits > 1 ? (float*)partial : nullptr;
     const dim3 grid(m.tiles_o * blocks_of(m.M, bt), splits);
-    if (bt == 128) hipLaunchKernelGGL((k_ad_gemm<T, 128>), grid, dim3(256), 0, st, m);
-    else hipLaunchKernelGGL((k_ad_gemm<T, 64>), grid, dim3(256), 0, st, m);
+    if (bt == 64) hipLaunchKernelGGL((k_ad_gemm<T, 64, 128>), grid, dim3(256), 0, st, m);
+    else if (rb == 128) hipLaunchKernelGGL((k_ad_gemm<T, 128, 128>), grid, dim3(256), 0, st, m);
+    else hipLaunchKernelGGL((k_ad_gemm<T, 128, 64>), grid, dim3(256), 0, st, m);
     HMF_LAUNCH_CHECK();
     if (splits > 1) {
         const long long n = (long long)m.M * m.O;
@@ -1172,7 +1195,7 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
         if (vec) hipLaunchKernelGGL((k_ad_few<T, true>), grid, dim3(256), 0, st, g, to, tm);
         else hipLaunchKernelGGL((k_ad_few<T, false>), grid, dim3(256), 0, st, g, to, tm);
         HMF_LAUNCH_CHECK();
-        hipLaunchKernelGGL(k_ad_join<T>, dim3(blocks_of((long long)M * N, 256)), dim3(256), 0, st, g);
+        hipLaunchKernelGGL(k_ad_join<T>, dim3(blocks_of((long long)M * N, 64)), dim3(64), 0, st, g);
         HMF_LAUNCH_CHECK();
         return HMF_OK;
     }
@@ -1261,8 +1284,7 @@ static int backward_t(const T* dy, const void* x, long long ldx, const unsigned 
     if (exps) hipLaunchKernelGGL((k_ad_grads<T, true>), grid, dim3(256), 0, st, ga, gb, order, seg, r, L);
     else hipLaunchKernelGGL((k_ad_grads<T, false>), grid, dim3(256), 0, st, ga, gb, order, seg, r, L);
     HMF_LAUNCH_CHECK();
-    const int wa = blocks_of((long long)r * K, 256), wb = blocks_of((long long)r * N, 256);
-    hipLaunchKernelGGL(k_ad_grad_join<T>, dim3(wa + wb, L), dim3(256), 0, st, ga, gb, seg, r, L, wa);
+    hipLaunchKernelGGL(k_ad_grad_join<T>, dim3(std::min(256, blocks_of((long long)r * (K + N), 256)), L), dim3(256), 0, st, ga, gb, seg, r, L);
     HMF_LAUNCH_CHECK();
     return HMF_OK;
 }
