@@ -458,11 +458,18 @@ __global__ __launch_bounds__(256) void k_bn8_finalize(const double* __restrict__
     }
 }
 
-template <bool GZ, bool NT>
+// What the second pass needs to add the partial sums itself (FOLD): every wave those of its 64 channels, 1 KB for each work-group of the first pass.
+struct Bn8Fold {
+    const double* part;
+    const float* gamma;
+    float *g_gamma, *g_beta;
+    int nparts;
+};
+template <bool GZ, bool NT, bool FOLD>
 __global__ __launch_bounds__(256) void k_bn8_apply(const float* __restrict__ g, const unsigned char* __restrict__ codes, const unsigned char* __restrict__ exps,
                                                    const unsigned int* __restrict__ bits, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                    const float* __restrict__ coef, float* __restrict__ gy, float* __restrict__ gz_out, int M, int C, int ct,
-                                                   long long tiles) {
+                                                   long long tiles, const Bn8Fold f) {
     // last tile first: the reduction ended there, and what it read last is still in the Infinity Cache
     const long long tile = tiles - 1 - ((long long)blockIdx.x * 4 + (threadIdx.x >> 6));
     if (tile < 0) return;
@@ -485,7 +492,38 @@ __global__ __launch_bounds__(256) void k_bn8_apply(const float* __restrict__ g, 
     if (bits) b = *(const uint4*)(bits + (long long)t * C + c);
     const unsigned int on[4] = {b.x >> q, b.y >> q, b.z >> q, b.w >> q};
     const f32x4 mu = *(const f32x4*)(mean + c), rs = *(const f32x4*)(rstd + c);
-    const f32x4 ca = *(const f32x4*)(coef + c), cs = *(const f32x4*)(coef + C + c), cx = *(const f32x4*)(coef + 2 * C + c);
+    f32x4 ca, cs, cx;
+    if (FOLD) {                                                            // lane = one of the wave's 64 channels, then handed to the lanes that use it
+        const int ch = c - (lane & 15) * 4 + lane;
+        double a = 0.0, b2 = 0.0;
+        for (int p0 = 0; p0 < f.nparts; p0 += 8) {
+            double v[8], x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const long long p = min(p0 + k, f.nparts - 1);
+                v[k] = f.part[p * 2 * C + ch];
+                x[k] = f.part[(p * 2 + 1) * C + ch];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (p0 + k < f.nparts) { a += v[k]; b2 += x[k]; }
+        }
+        const float fa = f.gamma[ch] * rstd[ch], fs = (float)(a / M), fx = (float)(b2 / M);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            ca[k] = __shfl(fa, (lane & 15) * 4 + k);
+            cs[k] = __shfl(fs, (lane & 15) * 4 + k);
+            cx[k] = __shfl(fx, (lane & 15) * 4 + k);
+        }
+        if (t == 0) {
+            f.g_beta[ch] = (float)a;
+            f.g_gamma[ch] = (float)b2;
+        }
+    } else {
+        ca = *(const f32x4*)(coef + c);
+        cs = *(const f32x4*)(coef + C + c);
+        cx = *(const f32x4*)(coef + 2 * C + c);
+    }
     float st[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) st[k] = step_of((int)((e >> (8 * k)) & 0xffu));
@@ -517,10 +555,11 @@ static int bn8_tiles_per_wg(int M, int C) {
     const int nt = (M + 31) / 32;
     const long long cols = C / 64;
     int per = (int)std::min<long long>(16, (nt * cols + 2047) / 2048);
-    per = std::max(4, (per + 3) / 4 * 4);
+    per = std::max(8, (per + 3) / 4 * 4);
     while ((long long)((nt + per - 1) / per) > 65535) per *= 2;                // the grid's y extent
     return per;
 }
+constexpr long long kFoldReads = 64 << 10;      // wave reads of 1 KB: 64 MB
 static int bn8_parts(int M, int C) { const int per = bn8_tiles_per_wg(M, C); return ((M + 31) / 32 + per - 1) / per; }
 
 static inline bool misaligned(const void* p, unsigned a) { return ((uintptr_t)p & (a - 1)) != 0; }
@@ -640,16 +679,23 @@ int hmf_bn_backward_act8(const float* g, const signed char* codes, const unsigne
     const unsigned char* cd = (const unsigned char*)codes;
     hipLaunchKernelGGL(k_bn8_reduce, dim3(ct, parts), dim3(256), 0, st, g, cd, exps, bits, mean, rstd, M, C, per, part);
     HMF_LAUNCH_CHECK();
-    hipLaunchKernelGGL(k_bn8_finalize, dim3(C / 4), dim3(256), 0, st, part, parts, M, C, gamma, rstd, g_gamma, g_beta, coef);
-    HMF_LAUNCH_CHECK();
     const long long tiles = (long long)((M + 31) / 32) * ct;
+    // A launch of its own for the partial sums costs 3 us and the call's host time another 3; adding them in every wave of the second pass costs their reads.
+    const bool fold = tiles * parts <= kFoldReads;
+    if (!fold) {
+        hipLaunchKernelGGL(k_bn8_finalize, dim3(C / 4), dim3(256), 0, st, part, parts, M, C, gamma, rstd, g_gamma, g_beta, coef);
+        HMF_LAUNCH_CHECK();
+    }
+    const Bn8Fold f{part, gamma, g_gamma, g_beta, parts};
     const dim3 grid((unsigned)((tiles + 3) / 4)), block(256);
     const bool nt = (long long)M * C * 4 > kStreamBytes;
-#define HMF_BN8A(GZ, NT) hipLaunchKernelGGL((k_bn8_apply<GZ, NT>), grid, block, 0, st, g, cd, exps, bits, mean, rstd, coef, gy, gz, M, C, ct, tiles)
-    if (gz && nt) HMF_BN8A(true, true);
-    else if (gz) HMF_BN8A(true, false);
-    else if (nt) HMF_BN8A(false, true);
-    else HMF_BN8A(false, false);
+#define HMF_BN8A(GZ, NT, FOLD) hipLaunchKernelGGL((k_bn8_apply<GZ, NT, FOLD>), grid, block, 0, st, g, cd, exps, bits, mean, rstd, coef, gy, gz, M, C, ct, tiles, f)
+    if (gz && nt) HMF_BN8A(true, true, false);                             // never folded: a streamed map has far too many tiles
+    else if (nt) HMF_BN8A(false, true, false);
+    else if (gz && fold) HMF_BN8A(true, false, true);
+    else if (gz) HMF_BN8A(true, false, false);
+    else if (fold) HMF_BN8A(false, false, true);
+    else HMF_BN8A(false, false, false);
 #undef HMF_BN8A
     HMF_LAUNCH_CHECK();
     return HMF_OK;
