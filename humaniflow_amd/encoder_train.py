@@ -206,6 +206,9 @@ class _ZeroPool:
 class _Saved:
     __slots__ = ('conv', 'bn', 'x', 'y', 'out', 'mean', 'rstd', 'relu', 'stride', 'stem', 'pooled', 'argmax', 'ck', 'bits')
 
+    def __init__(self):
+        self.ck = self.bits = None                                    # the 8-bit checkpoint of y and the ReLU's bits, where they are kept instead of y and out
+
 
 def _rows_of(t):
     """(B, C, H, W) channels_last -> its rows (B H W, C), a view."""
@@ -464,7 +467,6 @@ class EncoderTrainFn(torch.autograd.Function):
             """xin: the input map, kept: what the unit keeps of it for the backward pass -> (output map, what its readers keep of that)."""
             s = _Saved()
             s.conv, s.bn, s.x, s.relu, s.stride, s.stem = conv, bn, kept, relu, conv.stride[0], stem
-            s.ck = s.bits = None
             if stem:
                 B, C, H, W = xin.shape
                 OH, OW = (H - 1) // 2 + 1, (W - 1) // 2 + 1
