@@ -17,7 +17,14 @@ from . import _lib
 
 BLOCK = 32                      # rows that share an exponent
 
+MAX_ROWS = 0x7fffff00           # rows and columns are 32-bit numbers below
+
 _DTYPES = (torch.float32, torch.bfloat16)
+
+
+def _fits(M, C):
+    if M > MAX_ROWS or C > MAX_ROWS:
+        raise ValueError('humaniflow_amd: (%d, %d) rows: row and column numbers are 32-bit' % (M, C))
 
 
 class Act8:
@@ -32,6 +39,7 @@ class Act8:
             raise ValueError('humaniflow_amd: Act8: exps %s on %s do not fit codes %s on %s' % (tuple(exps.shape), exps.device, tuple(codes.shape), codes.device))
         if not (codes.is_contiguous() and exps.is_contiguous()):
             raise ValueError('humaniflow_amd: Act8 codes and exps must be contiguous')
+        _fits(M, C)
         self.shape, self.device, self._codes, self._exps, self._buf = codes.shape, codes.device, codes, exps, None
         self.codes_ptr, self.exps_ptr = codes.data_ptr(), exps.data_ptr()
 
@@ -82,6 +90,7 @@ def _rows(t, name, C=None, M=None):
     if t.dtype != torch.float32 or t.dim() != 2 or not t.is_contiguous() or (C is not None and t.shape[1] != C) or (M is not None and t.shape[0] != M):
         raise ValueError('humaniflow_amd: `%s` must be contiguous float32 rows%s, got %s %s' % (name, '' if C is None else ' (%d, %d)' % (M, C), t.dtype, tuple(t.shape)))
     _lib.require_cuda(t, name)
+    _fits(*t.shape)
 
 
 def _same_device(dev, **tensors):
@@ -110,6 +119,7 @@ def pack(x):
         raise ValueError('humaniflow_amd: act8.pack takes float32 or bfloat16 rows (M, C), got %s %s' % (x.dtype, tuple(x.shape)))
     x = x.detach()
     M, C = x.shape
+    _fits(M, C)
     if (C > 1 and x.stride(1) != 1) or (M > 1 and x.stride(0) < C):
         x = x.contiguous()
     ck = _in_buffer(torch.empty(_bytes_of(M, C), dtype=torch.uint8, device=x.device), 0, M, C)

@@ -34,6 +34,8 @@ def _check(x, weight, bias, A, B, scale, ids):
         raise ValueError('humaniflow_amd: adapted_linear: x %s, weight %s, A %s, B %s do not fit' % (tuple(xs), tuple(ws), tuple(As), tuple(Bs)))
     if r > MAX_RANK:
         raise ValueError('humaniflow_amd: adapters of rank %d: built up to %d' % (r, MAX_RANK))
+    if max(M, K, N, L) > act8.MAX_ROWS:
+        raise ValueError('humaniflow_amd: adapted_linear: x %s, weight %s, A %s: sizes are 32-bit' % (tuple(xs), tuple(ws), tuple(As)))
     if A.dtype != dt or B.dtype != dt or (bias is not None and (bias.dtype != dt or bias.shape != (N,))):
         raise ValueError('humaniflow_amd: adapted_linear: bias (%d), A and B must have the weight\'s type %s' % (N, dt))
     if scale.dtype != torch.float32 or scale.shape != (L,):

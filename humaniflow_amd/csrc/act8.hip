@@ -563,7 +563,8 @@ constexpr long long kFoldReads = 64 << 10;      // wave reads of 1 KB: 64 MB
 static int bn8_parts(int M, int C) { const int per = bn8_tiles_per_wg(M, C); return ((M + 31) / 32 + per - 1) / per; }
 
 static inline bool misaligned(const void* p, unsigned a) { return ((uintptr_t)p & (a - 1)) != 0; }
-constexpr long long kMaxTiles = 4LL * 0x7fffffff;                          // four tiles to a work-group, the grid's x extent
+constexpr long long kMaxTiles = 4LL * 16777215;                            // four tiles to a work-group of 256: a grid has under 2^32 threads
+constexpr int kMaxRows = 0x7fffff00;                                       // row numbers are ints
 
 }  // namespace hmf
 
@@ -578,8 +579,8 @@ int hmf_act8_pack(const void* x, long long ld, int bf16, int M, int C, signed ch
     const int V = bf16 ? 8 : 4;
     const bool fast = C % V == 0 && ld % V == 0 && !misaligned(x, 16) && !misaligned(codes, 4) && !misaligned(exps, 4);
     const int cols = fast ? 16 * V : 64, ct = (C + cols - 1) / cols;
-    const long long tiles = (long long)((M + 31) / 32) * ct;
-    if (tiles > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_act8_pack: M=%d C=%d exceeds the grid", M, C);
+    const long long tiles = ((long long)M + 31) / 32 * ct;
+    if (M > kMaxRows || tiles > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_act8_pack: M=%d C=%d exceeds the grid", M, C);
     const dim3 grid((unsigned)((tiles + 3) / 4)), block(256);
     hipStream_t st = (hipStream_t)stream;
     unsigned char* cd = (unsigned char*)codes;
@@ -598,8 +599,8 @@ int hmf_act8_unpack(const signed char* codes, const unsigned char* exps, int M, 
     const int V = bf16 ? 8 : 4;
     const bool fast = C % V == 0 && !misaligned(x, 16) && !misaligned(codes, 4) && !misaligned(exps, 4);
     const int cols = fast ? 16 * V : 64, ct = (C + cols - 1) / cols;
-    const long long tiles = (long long)((M + 31) / 32) * ct;
-    if (tiles > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_act8_unpack: M=%d C=%d exceeds the grid", M, C);
+    const long long tiles = ((long long)M + 31) / 32 * ct;
+    if (M > kMaxRows || tiles > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_act8_unpack: M=%d C=%d exceeds the grid", M, C);
     const dim3 grid((unsigned)((tiles + 3) / 4)), block(256);
     hipStream_t st = (hipStream_t)stream;
     const unsigned char* cd = (const unsigned char*)codes;
@@ -619,8 +620,8 @@ int hmf_bn_apply_act8(const float* y, const float* scale, const float* shift, co
         misaligned(exps, 4) || misaligned(bits, 16) || misaligned(out_codes, 4) || misaligned(out_exps, 4))
         return fail(HMF_ERR_INVALID, "hmf_bn_apply_act8: float tensors and bits must be 16-byte aligned, codes and exps 4-byte");
     const int ct = C / 64;
-    const long long tiles = (long long)((M + 31) / 32) * ct;
-    if (tiles > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_bn_apply_act8: M=%d C=%d exceeds the grid", M, C);
+    const long long tiles = ((long long)M + 31) / 32 * ct;
+    if (M > kMaxRows || tiles > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_bn_apply_act8: M=%d C=%d exceeds the grid", M, C);
     const dim3 grid((unsigned)((tiles + 3) / 4)), block(256);
     hipStream_t st = (hipStream_t)stream;
     unsigned char *cd = (unsigned char*)codes, *oc = (unsigned char*)out_codes;
@@ -648,8 +649,8 @@ int hmf_act8_restore_activation(const signed char* codes, const unsigned char* e
     if (misaligned(codes, 4) || misaligned(exps, 4) || misaligned(bits, 16) || misaligned(scale, 16) || misaligned(shift, 16) || misaligned(x, 16))
         return fail(HMF_ERR_INVALID, "hmf_act8_restore_activation: float tensors and bits must be 16-byte aligned, codes and exps 4-byte");
     const int ct = C / 64;
-    const long long tiles = (long long)((M + 31) / 32) * ct;
-    if (tiles > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_act8_restore_activation: M=%d C=%d exceeds the grid", M, C);
+    const long long tiles = ((long long)M + 31) / 32 * ct;
+    if (M > kMaxRows || tiles > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_act8_restore_activation: M=%d C=%d exceeds the grid", M, C);
     hipLaunchKernelGGL(k_act8_restore, dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, (hipStream_t)stream, (const unsigned char*)codes, exps, bits, scale, shift,
                        x, M, C, ct, tiles);
     HMF_LAUNCH_CHECK();
@@ -657,7 +658,7 @@ int hmf_act8_restore_activation(const signed char* codes, const unsigned char* e
 }
 
 size_t hmf_bn_backward_act8_workspace_bytes(int M, int C) {
-    if (M <= 0 || C <= 0 || C % 64) return 0;
+    if (M <= 0 || M > kMaxRows || C <= 0 || C % 64) return 0;
     return (size_t)bn8_parts(M, C) * 2 * C * sizeof(double) + (size_t)3 * C * sizeof(float);
 }
 
@@ -672,14 +673,14 @@ int hmf_bn_backward_act8(const float* g, const signed char* codes, const unsigne
     const size_t need = hmf_bn_backward_act8_workspace_bytes(M, C);
     if (!workspace || workspace_bytes < need) return fail(HMF_ERR_WORKSPACE, "hmf_bn_backward_act8: workspace %zu < %zu bytes", workspace_bytes, need);
     const int per = bn8_tiles_per_wg(M, C), parts = bn8_parts(M, C), ct = C / 64;
-    if ((long long)((M + 31) / 32) * ct > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_bn_backward_act8: M=%d C=%d exceeds the grid", M, C);
+    if (M > kMaxRows || (long long)((M + 31) / 32) * ct > kMaxTiles) return fail(HMF_ERR_UNSUPPORTED, "hmf_bn_backward_act8: M=%d C=%d exceeds the grid", M, C);
     double* part = (double*)workspace;
     float* coef = (float*)(part + (size_t)parts * 2 * C);
     hipStream_t st = (hipStream_t)stream;
     const unsigned char* cd = (const unsigned char*)codes;
     hipLaunchKernelGGL(k_bn8_reduce, dim3(ct, parts), dim3(256), 0, st, g, cd, exps, bits, mean, rstd, M, C, per, part);
     HMF_LAUNCH_CHECK();
-    const long long tiles = (long long)((M + 31) / 32) * ct;
+    const long long tiles = ((long long)M + 31) / 32 * ct;
     // A launch of its own for the partial sums costs 3 us and the call's host time another 3; adding them in every wave of the second pass costs their reads.
     const bool fold = tiles * parts <= kFoldReads;
     if (!fold) {

@@ -1141,10 +1141,12 @@ static BwdWs bwd_ws(int M, int K, int N, int r, int L, size_t z) {
 static int check_sizes(const char* who, int M, int K, int N, int r, int L) {
     if (M < 0 || K < 1 || N < 1 || r < 1 || L < 1) return fail(HMF_ERR_INVALID, "%s: M=%d K=%d N=%d r=%d L=%d", who, M, K, N, r, L);
     if (r > kMaxRank) return fail(HMF_ERR_UNSUPPORTED, "%s: rank %d, built up to %d", who, r, kMaxRank);
-    const long long tk = blocks_of(K, 32) + 2, tn = blocks_of(N, 32) + 2;    // 32 x 32 tiles of the copies (padded rows)
-    if (L > 65535 || (long long)L + M / kFewRows > 65535 || (long long)L * r > 0x3fffffffLL || blocks_of(M, 32) * std::max(tk, tn) > 0x1fffffffLL || tk * tn > 0x1fffffffLL ||
-        blocks_of((long long)L * r, 32) * std::max(tk, tn) > 0x1fffffffLL || (long long)L * blocks_of(r, 32) * tn > 0x1fffffffLL)
-        return fail(HMF_ERR_UNSUPPORTED, "%s: M=%d K=%d N=%d L=%d exceed the grid", who, M, K, N, L);
+    // a grid has under 2^32 threads in a dimension, and its y extent is 16 bits
+    const long long c = std::max(K, N) + 128ll, tc = c / 64 + 1, most = 4194303;                      // work-groups of 1,024
+    const bool few = M <= kFewRows;
+    if (L > 65535 || (long long)L + M / kFewRows > 65535 || (few && M * c > 0xffffff00ll) ||
+        (!few && (long long)L + 1 + (M / 64 + 1) * tc + (N / 64 + 1) * (long long)(K / 64 + 3) + std::max((long long)L * r / 64 + 1, (long long)L) * tc > most))
+        return fail(HMF_ERR_UNSUPPORTED, "%s: M=%d K=%d N=%d r=%d L=%d exceed the grid", who, M, K, N, r, L);
     return HMF_OK;
 }
 

@@ -16,8 +16,9 @@ from .smpl import compute_vertex_variance_from_samples
 
 
 @torch.no_grad()
-def predict_humaniflow(humaniflow_model, smpl_model, proxy_inputs, names, save_dir=None, num_pred_samples=50, noise=None):
-    """proxy_inputs: (B, 18, S, S) on the model's device; processed one image at a time like the reference loop (:65)."""
+def predict_humaniflow(humaniflow_model, smpl_model, proxy_inputs, names, save_dir=None, num_pred_samples=50, noise=None, adapter_ids=None):
+    """proxy_inputs: (B, 18, S, S) on the model's device; processed one image at a time like the reference loop (:65).  adapter_ids (B,): each image's own
+    low-rank adapter of the model's heads (HumaniflowModel.attach_adapters)."""
     humaniflow_model.eval()
     humaniflow_model.pose_so3flow_transform_modules.eval()                                    # :60-61
     results = []
@@ -25,7 +26,8 @@ def predict_humaniflow(humaniflow_model, smpl_model, proxy_inputs, names, save_d
     for i, name in enumerate(names):
         x = proxy_inputs[i:i + 1]
         nz = None if noise is None else {k: v[:, i:i + 1].contiguous() for k, v in noise.items()}
-        pred = humaniflow_model(x, num_samples=N, use_shape_mode_for_samples=True, return_input_feats=True, noise=nz)   # :112-115
+        pred = humaniflow_model(x, num_samples=N, use_shape_mode_for_samples=True, return_input_feats=True, noise=nz,   # :112-115
+                                adapter_ids=None if adapter_ids is None else adapter_ids[i:i + 1])
         out_np = {k: pred[k].cpu().numpy()[0] for k in ('pose_axisangle_point_est', 'pose_rotmats_point_est', 'shape_mode',
                                                           'glob_rotmat', 'cam_wp', 'input_feats')}          # predict_utils.py:19-24
         if save_dir is not None:

@@ -53,12 +53,13 @@ def _side_stream(device):
     return _SIDE[key]
 
 
-def train_forward_loss(model, smpl, criterion, proxy_input, targets, num_samples, noise=None, input_feats=None):
+def train_forward_loss(model, smpl, criterion, proxy_input, targets, num_samples, noise=None, input_feats=None, adapter_ids=None):
     """targets: pose_rotmats (B,23,3,3), glob_rotmats (B,3,3), shape (B,nb), joints2D (B,17,2) pixels, joints2D_vis (B,17) bool.
-    Returns (loss, pred).  J2D_LOSS_ON = 'point_est+samples' | 'samples' | 'point_est' as LOSS.J2D_LOSS_ON."""
+    adapter_ids (B,): the images' own low-rank adapters (model.attach_adapters), for fitting those.  Returns (loss, pred).  J2D_LOSS_ON = 'point_est+samples' | 'samples' | 'point_est' as LOSS.J2D_LOSS_ON."""
     N = num_samples
     pred = model(proxy_input, compute_point_est=True, num_samples=N, compute_for_loglik=True, shape_for_loglik=targets['shape'],
-                 pose_R_for_loglik=targets['pose_rotmats'], glob_R_for_loglik=targets['glob_rotmats'], noise=noise, input_feats=input_feats)
+                 pose_R_for_loglik=targets['pose_rotmats'], glob_R_for_loglik=targets['glob_rotmats'], noise=noise, input_feats=input_feats,
+                 adapter_ids=adapter_ids)
     B = pred['glob_rotmat'].shape[0]
     cfg_l = criterion.loss_cfg
     dists = pred['conditioned_pose_SO3flow_dists_for_loglik']
@@ -319,7 +320,7 @@ def nans_in_output(pred):
     return torch.stack(flags).any() if flags else torch.zeros((), dtype=torch.bool)
 
 
-def train_step(model, smpl, criterion, optimiser, reducer, proxy_input, targets, num_samples, noise=None, nan_policy='skip', last_state=None):
+def train_step(model, smpl, criterion, optimiser, reducer, proxy_input, targets, num_samples, noise=None, nan_policy='skip', last_state=None, adapter_ids=None):
     """One optimisation step.  Returns (loss tensor, skipped): a non-finite loss or gradient skips the update (the reference reloads the previous
     state dicts, train/train_humaniflow.py:264-278).  With a fused Adam on the device the decision never leaves the device: the finite flag is
     handed to the optimiser as `found_inf` (the fused kernel then leaves parameters, moments and step counts untouched), `skipped` is a 0-dim
@@ -340,7 +341,7 @@ def train_step(model, smpl, criterion, optimiser, reducer, proxy_input, targets,
         raise ValueError("nan_policy='rollback' needs last_state=LastBatchState(model, optimiser), kept across steps")
     optimiser.zero_grad(set_to_none=True)
     reducer.begin()
-    loss, pred = train_forward_loss(model, smpl, criterion, proxy_input, targets, num_samples, noise=noise)
+    loss, pred = train_forward_loss(model, smpl, criterion, proxy_input, targets, num_samples, noise=noise, adapter_ids=adapter_ids)
     if nan_policy == 'rollback':
         nan = nans_in_output(pred)
         if reducer.world > 1:                                           # every rank must take the same branch
@@ -351,7 +352,7 @@ def train_step(model, smpl, criterion, optimiser, reducer, proxy_input, targets,
             print('Re-doing current batch forward pass.')
             del loss, pred
             reducer.begin()
-            loss, pred = train_forward_loss(model, smpl, criterion, proxy_input, targets, num_samples, noise=noise)
+            loss, pred = train_forward_loss(model, smpl, criterion, proxy_input, targets, num_samples, noise=noise, adapter_ids=adapter_ids)
         last_state.save()
     loss.backward()
     reducer.finish()

@@ -79,6 +79,7 @@ def test_refusals_of_the_c_entry_points(lib):
     assert lib.hmf_act8_pack(n, 4, 0, 0, 4, n, n, n) == 0                       # no rows: nothing to do
     assert lib.hmf_act8_unpack(p, p, 2, -3, p, 0, n) == -1
     assert lib.hmf_act8_unpack(p, n, 2, 3, p, 0, n) == -1
+    assert lib.hmf_act8_pack(p, 4, 0, 0x7fffffff, 4, p, p, n) == -2 and lib.hmf_act8_unpack(p, p, 0x7fffff00, 0x7fffff00, p, 0, n) == -2
     bn = lambda y=p, bits=p, oc=n, oe=n, M=2, Cn=64, relu=1: lib.hmf_bn_apply_act8(y, p, p, n, p, p, p, bits, oc, oe, M, Cn, relu, n)
     assert bn(Cn=63) == -1 and bn(M=0) == -1 and bn(y=n) == -1 and bn(bits=n) == -1 and bn(relu=0) == -1 and bn(oc=p) == -1 and bn(oe=p) == -1
     assert bn(y=odd) == -1 and b'aligned' in lib.hmf_last_error()

@@ -63,6 +63,7 @@ def test_refusals_of_the_c_entry_points(lib):
     assert need > 0 and fw(M=0) == 0
     assert fw(x=n) == -1 and fw(ldx=5) == -1 and fw(K=0) == -1 and fw(M=-1) == -1 and fw(L=0) == -1 and fw(r=0) == -1
     assert fw(r=65) == -2 and fw(L=70000) == -2
+    assert fw(M=256, N=1 << 25) == -2 and fw(M=1 << 25) == -2 and b'grid' in lib.hmf_last_error()
     assert fw(ws=n) == -4 and fw(nb=need - 1) == -4 and fw(ws=C.c_void_p(p.value + 4)) == -4
     need = lib.hmf_adapted_linear_backward_workspace_bytes(4, 6, 3, 2, 2, 0)
     bw = lambda dy=p, ldx=6, exps=n, M=4, r=2, ws=p, nb=1 << 20: lib.hmf_adapted_linear_backward(dy, p, ldx, exps, p, p, p, p, p, p, M, 6, 3, r, 2, 0, p, p, p, ws, nb, n)

@@ -273,3 +273,34 @@ def test_encoder_refuses_an_unknown_checkpoint():
     enc.activation_checkpoint = 'fp8'
     with pytest.raises(ValueError, match='activation_checkpoint'):
         enc(torch.randn(1, 18, 64, 64, device='cuda'))
+
+
+def test_captured_training_pass_with_int8_checkpoints():
+    """Forward and backward of the encoder in one graph, replayed with other inputs and the program's own work between; the weight gradients' sums use float atomics, so
+    they are compared within 1e-4 of their norm."""
+    torch.manual_seed(1)
+    enc = ResNetEncoder(18, 18).cuda().train()
+    enc.activation_checkpoint = 'int8'
+    x, w = torch.randn(4, 18, 64, 64, device='cuda'), torch.randn(4, 512, device='cuda')
+
+    def step():
+        f = enc(x)
+        return (f, *torch.autograd.grad((f * w).sum(), list(enc.parameters())))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(3):
+        x.copy_(torch.randn_like(x))
+        w.mul_(0.7)
+        graph.replay()
+        got = [t.detach().clone() for t in held]
+        want = [t.detach() for t in step()]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert (a - b).norm().item() <= 1e-4 * b.norm().item() + 1e-12, k

@@ -327,3 +327,70 @@ def test_model_refusals():
         model(None, input_feats=feats, adapter_ids=ids[:2])
     with pytest.raises(RuntimeError, match='fixed projection'):
         model.train()(None, input_feats=feats, adapter_ids=ids)
+
+
+def test_predict_takes_each_images_adapter():
+    from humaniflow_amd.predict import predict_humaniflow
+    model = _model()
+    ad = H.LowRankAdapters(model, 2, 4)
+    with torch.no_grad():
+        ad.fc1_B.normal_(0, 0.05)
+        ad.fc_shape_B.normal_(0, 0.05)
+    model.attach_adapters(ad)
+    smpl = H.SMPL(model_data=H.synthetic_smpl_model(seed=0), create_transl=False).cuda()
+    x, ids = torch.randn(3, 18, 64, 64, device='cuda'), torch.tensor([1, -1, 0], device='cuda')
+    res = predict_humaniflow(model, smpl, x, ['a', 'b', 'c'], num_pred_samples=0, adapter_ids=ids)
+    plain = predict_humaniflow(model, smpl, x, ['a', 'b', 'c'], num_pred_samples=0)
+    with torch.no_grad():
+        for i in range(3):
+            ref = model(x[i:i + 1], adapter_ids=ids[i:i + 1])
+            assert torch.equal(res[i]['pred']['shape_mode'], ref['shape_mode'])
+            same = (res[i]['pred']['shape_mode'] - plain[i]['pred']['shape_mode']).abs().max().item() < 1e-5
+            assert same == (i == 1)
+
+
+def test_training_step_fits_adapters():
+    """train.train_step with adapter_ids: the heads' adapters and the encoder (8-bit checkpoints) move, the shared heads do not, adapters nobody used keep their values."""
+    from humaniflow_amd import train as T
+    from humaniflow_amd.synthetic import init_benchmark_weights
+    cfg = H.get_humaniflow_cfg_defaults()
+    model = init_benchmark_weights(H.HumaniflowModel(torch.device('cpu'), cfg.MODEL, H.SMPL_PARENTS), seed=0).cuda()
+    for name in ('fc1', 'fc_cam', 'fc_glob', 'fc_shape'):
+        getattr(model, name).requires_grad_(False)
+    model.attach_adapters(H.LowRankAdapters(model, 3, 4, checkpoint='int8'))
+    model.image_encoder.activation_checkpoint = 'int8'
+    model.train()
+    smpl = H.SMPL(model_data=H.synthetic_smpl_model(seed=0), batch_size=4, create_transl=False).cuda()
+    for p in smpl.parameters():
+        p.requires_grad_(False)
+    params = [p for p in model.parameters() if p.requires_grad]
+    opt = torch.optim.SGD(params, lr=1e-4)
+    red = T.GradBucketReducer(params, None)
+    batch = T.synthetic_train_batch(smpl, 4, 128, torch.device('cuda'), seed=1, data_cfg=cfg.DATA)
+    ids = torch.tensor([0, 1, -1, 0], device='cuda')
+    crit = H.HumaniflowLoss(cfg.LOSS, 128)
+    before = {n: p.detach().clone() for n, p in model.named_parameters()}
+    for _ in range(2):
+        loss, skipped = T.train_step(model, smpl, crit, opt, red, *batch, 2, adapter_ids=ids)
+        assert torch.isfinite(loss) and not skipped
+    moved = {n for n, p in model.named_parameters() if not torch.equal(before[n], p)}
+    assert {'adapters.fc1_B', 'adapters.fc_shape_B', 'adapters.fc1_A', 'image_encoder.conv1.weight'} <= moved
+    assert not moved & {'fc1.weight', 'fc1.bias', 'fc_cam.weight', 'fc_glob.weight', 'fc_shape.weight'}
+    assert torch.equal(before['adapters.fc1_B'][2], model.adapters.fc1_B[2]) and torch.equal(before['adapters.fc1_A'][2], model.adapters.fc1_A[2])
+
+
+@pytest.mark.parametrize('M', [7, 300])
+def test_gradient_of_a_broadcast_input_and_of_shared_adapters(M):
+    """One row used by every request, and one pair of adapters used by two layers: the gradients add up."""
+    c = _case(M, 64, 64, 4, 3, 'mixed', torch.float32, 8)
+    row = c['x'][:1].clone().requires_grad_(True)
+    A, B = c['A'].clone().requires_grad_(True), c['B'].clone().requires_grad_(True)
+    args = (c['weight'], c['bias'], A, B, c['scale'], c['ids'])
+    h = adapters.adapted_linear(row.expand(M, 64), *args)
+    adapters.adapted_linear(h, *args).sum().backward()
+    d = [t.detach().double().requires_grad_(True) for t in (c['x'][:1], A, B)]
+    on, l = (c['ids'] >= 0).double()[:, None], c['ids'].clamp(min=0).long()
+    f = lambda v: v @ c['weight'].double().t() + c['bias'].double() + on * c['scale'].double()[l][:, None] * torch.matmul(d[2][l], torch.matmul(d[1][l], v[:, :, None]))[:, :, 0]
+    f(f(d[0].expand(M, 64))).sum().backward()
+    for got, ref in zip((row, A, B), d):                                  # sums of up to 300 rows of 64-term products in 32 bits: 1e-5 of the norm is 40 times their walk
+        assert (got.grad.double() - ref.grad).norm().item() <= 1e-5 * ref.grad.norm().item()
