@@ -278,25 +278,12 @@ def dptr(t):
     return t.data_ptr()
 
 
-class on_device:
-    """`with on_device(dev) as st:` -- dev is the current device inside, st its current stream as the C entry points take it.  The device is switched only where
-    it differs, and the stream is asked for without building a torch.cuda.Stream: a small launch's host time is mostly such things."""
-    __slots__ = ('guard', 'index')
-
-    def __init__(self, device):
-        import torch
-        cur = torch._C._cuda_getDevice()
-        self.index = cur if device.index is None else device.index
-        self.guard = None if self.index == cur else torch.cuda.device(self.index)
-
-    def __enter__(self):
-        import torch
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        return self.guard.__exit__(*exc) if self.guard is not None else False
+def stream_here(device):
+    """`device`'s current stream as the C entry points take it if `device` is the current one, else None: the caller then calls itself under
+    torch.cuda.device(device).  No torch.cuda.Stream is built and no device is switched to itself: a small launch's host time is mostly such things."""
+    import torch
+    cur = torch._C._cuda_getDevice()
+    return torch._C._cuda_getCurrentRawStream(cur) if device.index == cur else None
 
 
 def current_stream():

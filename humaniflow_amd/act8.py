@@ -71,12 +71,12 @@ def _bytes_of(M, C):
     return _round16(M * C) + _round16((M + BLOCK - 1) // BLOCK * C)
 
 
-def _in_buffer(buf, at, M, C):
-    """The checkpoint of (M, C) rows whose codes and exponents lie (or will lie) at byte `at` of buf."""
+def _in_buffer(buf, at, shape, device):
+    """The checkpoint of rows of `shape` whose codes and exponents lie (or will lie) at byte `at` of buf."""
     ck = Act8.__new__(Act8)
-    ck.shape, ck.device, ck._codes, ck._exps, ck._buf, ck._at = torch.Size((M, C)), buf.device, None, None, buf, at
+    ck.shape, ck.device, ck._codes, ck._exps, ck._buf, ck._at = shape, device, None, None, buf, at
     ck.codes_ptr = buf.data_ptr() + at
-    ck.exps_ptr = ck.codes_ptr + _round16(M * C)
+    ck.exps_ptr = ck.codes_ptr + _round16(shape[0] * shape[1])
     return ck
 
 
@@ -99,33 +99,40 @@ def _same_device(dev, **tensors):
             raise ValueError('humaniflow_amd: `%s` is on %s, the other operands on %s' % (name, t.device, dev))
 
 
-def _channels(C, **vectors):
+def _channels(C, *named):
     if C % 64 or C == 0:
         raise ValueError('humaniflow_amd: the BatchNorm kernels are built for multiples of 64 channels, got %d' % C)
-    for name, v in vectors.items():
-        if v.dtype != torch.float32 or v.dim() != 1 or v.shape[0] != C or not v.is_contiguous():
+    for name, v in named:
+        if v.dtype != torch.float32 or v.shape != (C,) or not v.is_contiguous():
             raise ValueError('humaniflow_amd: `%s` must be a contiguous float32 vector of %d channels, got %s %s' % (name, C, v.dtype, tuple(v.shape)))
 
 
 def _check_bits(bits, M, C):
-    if bits is not None and (bits.dtype != torch.int32 or tuple(bits.shape) != ((M + BLOCK - 1) // BLOCK, C) or not bits.is_contiguous()):
+    if bits is not None and (bits.dtype != torch.int32 or bits.shape != ((M + BLOCK - 1) // BLOCK, C) or not bits.is_contiguous()):
         raise ValueError('humaniflow_amd: `bits` must be contiguous int32 (%d, %d), got %s %s' % ((M + BLOCK - 1) // BLOCK, C, bits.dtype, tuple(bits.shape)))
 
 
 def pack(x):
     """Checkpoint of x (M, C), float32 or bfloat16; rows may be strided (a view of wider rows), columns consecutive."""
-    _lib.require_cuda(x, 'x')
+    if not x.is_cuda:
+        _lib.require_cuda(x, 'x')
     if x.dtype not in _DTYPES or x.dim() != 2:
         raise ValueError('humaniflow_amd: act8.pack takes float32 or bfloat16 rows (M, C), got %s %s' % (x.dtype, tuple(x.shape)))
-    x = x.detach()
+    dev = x.device
+    st = _lib.stream_here(dev)
+    if st is None:
+        with torch.cuda.device(dev):
+            return pack(x)
     M, C = x.shape
     _fits(M, C)
-    if (C > 1 and x.stride(1) != 1) or (M > 1 and x.stride(0) < C):
-        x = x.contiguous()
-    ck = _in_buffer(torch.empty(_bytes_of(M, C), dtype=torch.uint8, device=x.device), 0, M, C)
-    lib = _lib.load()
-    with _lib.on_device(x.device) as st:
-        _lib.check(lib.hmf_act8_pack(x.data_ptr(), x.stride(0) if M > 1 else C, int(x.dtype == torch.bfloat16), M, C, ck.codes_ptr, ck.exps_ptr, st), 'hmf_act8_pack')
+    ld = C
+    if not x.is_contiguous():
+        if (C > 1 and x.stride(1) != 1) or (M > 1 and x.stride(0) < C):
+            x = x.detach().contiguous()
+        elif M > 1:
+            ld = x.stride(0)
+    ck = _in_buffer(torch.empty(_bytes_of(M, C), dtype=torch.uint8, device=dev), 0, x.shape, dev)
+    _lib.check(_lib.load().hmf_act8_pack(x.data_ptr(), ld, int(x.dtype == torch.bfloat16), M, C, ck.codes_ptr, ck.exps_ptr, st), 'hmf_act8_pack')
     return ck
 
 
@@ -134,11 +141,13 @@ def unpack(ck, dtype=torch.float32):
     if dtype not in _DTYPES:
         raise ValueError('humaniflow_amd: act8.unpack gives float32 or bfloat16, not %s' % dtype)
     _on_gpu(ck)
+    st = _lib.stream_here(ck.device)
+    if st is None:
+        with torch.cuda.device(ck.device):
+            return unpack(ck, dtype)
     M, C = ck.shape
-    x = torch.empty((M, C), dtype=dtype, device=ck.device)
-    lib = _lib.load()
-    with _lib.on_device(x.device) as st:
-        _lib.check(lib.hmf_act8_unpack(ck.codes_ptr, ck.exps_ptr, M, C, x.data_ptr(), int(dtype == torch.bfloat16), st), 'hmf_act8_unpack')
+    x = torch.empty(ck.shape, dtype=dtype, device=ck.device)
+    _lib.check(_lib.load().hmf_act8_unpack(ck.codes_ptr, ck.exps_ptr, M, C, x.data_ptr(), int(dtype == torch.bfloat16), st), 'hmf_act8_unpack')
     return x
 
 
@@ -147,21 +156,24 @@ def bn_apply(y, scale, shift, residual=None, relu=True, keep_out=False):
     checkpoint of out: (out, ck, bits, ck_out).  C a multiple of 64, M >= 1."""
     _rows(y, 'y')
     M, C = y.shape
-    _channels(C, scale=scale, shift=shift)
+    _channels(C, ('scale', scale), ('shift', shift))
     if residual is not None:
         _rows(residual, 'residual', C, M)
     dev = y.device
-    _same_device(dev, scale=scale, shift=shift, residual=residual)
+    if scale.device != dev or shift.device != dev or (residual is not None and residual.device != dev):
+        _same_device(dev, scale=scale, shift=shift, residual=residual)
+    st = _lib.stream_here(dev)
+    if st is None:
+        with torch.cuda.device(dev):
+            return bn_apply(y, scale, shift, residual, relu, keep_out)
     out = torch.empty_like(y)
     n = _bytes_of(M, C)
     buf = torch.empty(2 * n if keep_out else n, dtype=torch.uint8, device=dev)
-    ck, ck_out = _in_buffer(buf, 0, M, C), _in_buffer(buf, n, M, C) if keep_out else None
+    ck, ck_out = _in_buffer(buf, 0, y.shape, dev), _in_buffer(buf, n, y.shape, dev) if keep_out else None
     bits = torch.empty(((M + BLOCK - 1) // BLOCK, C), dtype=torch.int32, device=dev) if relu else None
-    lib = _lib.load()
-    with _lib.on_device(dev) as st:
-        _lib.check(lib.hmf_bn_apply_act8(y.data_ptr(), scale.data_ptr(), shift.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(),
-                                         ck.codes_ptr, ck.exps_ptr, None if bits is None else bits.data_ptr(), ck_out.codes_ptr if keep_out else None,
-                                         ck_out.exps_ptr if keep_out else None, M, C, int(relu), st), 'hmf_bn_apply_act8')
+    _lib.check(_lib.load().hmf_bn_apply_act8(y.data_ptr(), scale.data_ptr(), shift.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(),
+                                             ck.codes_ptr, ck.exps_ptr, None if bits is None else bits.data_ptr(), ck_out.codes_ptr if keep_out else None,
+                                             ck_out.exps_ptr if keep_out else None, M, C, int(relu), st), 'hmf_bn_apply_act8')
     return out, ck, bits, ck_out
 
 
@@ -170,14 +182,18 @@ def restore_activation(ck, scale, shift, bits=None):
     the affine alone)."""
     _on_gpu(ck)
     M, C = ck.shape
-    _channels(C, scale=scale, shift=shift)
+    _channels(C, ('scale', scale), ('shift', shift))
     _check_bits(bits, M, C)
-    _same_device(ck.device, scale=scale, shift=shift, bits=bits)
-    x = torch.empty((M, C), dtype=torch.float32, device=ck.device)
-    lib = _lib.load()
-    with _lib.on_device(x.device) as st:
-        _lib.check(lib.hmf_act8_restore_activation(ck.codes_ptr, ck.exps_ptr, None if bits is None else bits.data_ptr(), scale.data_ptr(),
-                                                   shift.data_ptr(), x.data_ptr(), M, C, st), 'hmf_act8_restore_activation')
+    dev = ck.device
+    if scale.device != dev or shift.device != dev or (bits is not None and bits.device != dev):
+        _same_device(dev, scale=scale, shift=shift, bits=bits)
+    st = _lib.stream_here(dev)
+    if st is None:
+        with torch.cuda.device(dev):
+            return restore_activation(ck, scale, shift, bits)
+    x = torch.empty(ck.shape, dtype=torch.float32, device=dev)
+    _lib.check(_lib.load().hmf_act8_restore_activation(ck.codes_ptr, ck.exps_ptr, None if bits is None else bits.data_ptr(), scale.data_ptr(), shift.data_ptr(),
+                                                       x.data_ptr(), M, C, st), 'hmf_act8_restore_activation')
     return x
 
 
@@ -185,20 +201,24 @@ def bn_backward(g, ck, bits, mean, rstd, gamma, want_gz=False):
     """g = dL/d out of a bn_apply (M, C) -> (gy = dL/dy, gz = the masked gradient or None, dL/d gamma, dL/d beta); bits None: no ReLU."""
     _rows(g, 'g')
     M, C = g.shape
-    _channels(C, mean=mean, rstd=rstd, gamma=gamma)
+    _channels(C, ('mean', mean), ('rstd', rstd), ('gamma', gamma))
     if ck.shape != g.shape:
         raise ValueError('humaniflow_amd: the checkpoint holds %s rows, the gradient is %s' % (tuple(ck.shape), (M, C)))
     _check_bits(bits, M, C)
     dev = g.device
-    _same_device(dev, checkpoint=ck, bits=bits, mean=mean, rstd=rstd, gamma=gamma)
+    if ck.device != dev or mean.device != dev or rstd.device != dev or gamma.device != dev or (bits is not None and bits.device != dev):
+        _same_device(dev, checkpoint=ck, bits=bits, mean=mean, rstd=rstd, gamma=gamma)
+    st = _lib.stream_here(dev)
+    if st is None:
+        with torch.cuda.device(dev):
+            return bn_backward(g, ck, bits, mean, rstd, gamma, want_gz)
     gy = torch.empty_like(g)
     gz = torch.empty_like(g) if want_gz else None
     gg, gb = torch.empty_like(gamma), torch.empty_like(gamma)
     lib = _lib.load()
-    n = int(lib.hmf_bn_backward_act8_workspace_bytes(M, C))
+    n = lib.hmf_bn_backward_act8_workspace_bytes(M, C)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev) as st:
-        _lib.check(lib.hmf_bn_backward_act8(g.data_ptr(), ck.codes_ptr, ck.exps_ptr, None if bits is None else bits.data_ptr(), mean.data_ptr(),
-                                            rstd.data_ptr(), gamma.data_ptr(), gy.data_ptr(), None if gz is None else gz.data_ptr(), gg.data_ptr(), gb.data_ptr(),
-                                            M, C, ws.data_ptr(), n, st), 'hmf_bn_backward_act8')
+    _lib.check(lib.hmf_bn_backward_act8(g.data_ptr(), ck.codes_ptr, ck.exps_ptr, None if bits is None else bits.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                        gamma.data_ptr(), gy.data_ptr(), None if gz is None else gz.data_ptr(), gg.data_ptr(), gb.data_ptr(), M, C, ws.data_ptr(), n,
+                                        st), 'hmf_bn_backward_act8')
     return gy, gz, gg, gb

@@ -77,16 +77,18 @@ def adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t=True):
     x, ldx = _rows(x)
     weight, bias, A, B, scale = _dense(weight), _dense(bias), _dense(A), _dense(B), _dense(scale)
     dev = weight.device
+    st = _lib.stream_here(dev)
+    if st is None:
+        with torch.cuda.device(dev):
+            return adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t)
     y = torch.empty((M, N), dtype=weight.dtype, device=dev)
     t = torch.empty((M, r), dtype=torch.float32, device=dev) if need_t else None
     lib = _lib.load()
     bf16 = int(weight.dtype == torch.bfloat16)
     n = lib.hmf_adapted_linear_workspace_bytes(M, K, N, r, L, bf16)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev) as st:
-        _lib.check(lib.hmf_adapted_linear(x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(),
-                                          ids.data_ptr(), M, K, N, r, L, bf16, y.data_ptr(), None if t is None else t.data_ptr(), ws.data_ptr(), n, st),
-                   'hmf_adapted_linear')
+    _lib.check(lib.hmf_adapted_linear(x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(),
+                                      ids.data_ptr(), M, K, N, r, L, bf16, y.data_ptr(), None if t is None else t.data_ptr(), ws.data_ptr(), n, st), 'hmf_adapted_linear')
     return y, t
 
 
@@ -112,17 +114,19 @@ def adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=True):
     else:
         x, ldx = _rows(x)
         xp, exps = x.data_ptr(), None
+    st = _lib.stream_here(dev)
+    if st is None:
+        with torch.cuda.device(dev):
+            return adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx)
     dx = torch.empty((M, K), dtype=dt, device=dev) if need_dx else None
     dA, dB = torch.empty_like(A), torch.empty_like(B)
     lib = _lib.load()
     bf16 = int(dt == torch.bfloat16)
     n = lib.hmf_adapted_linear_backward_workspace_bytes(M, K, N, r, L, bf16)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev) as st:
-        _lib.check(lib.hmf_adapted_linear_backward(dy.data_ptr(), xp, ldx, exps, t.data_ptr(), weight.data_ptr(),
-                                                   A.data_ptr(), B.data_ptr(), scale.data_ptr(), ids.data_ptr(), M, K, N, r, L, bf16,
-                                                   None if dx is None else dx.data_ptr(), dA.data_ptr(), dB.data_ptr(), ws.data_ptr(), n, st),
-                   'hmf_adapted_linear_backward')
+    _lib.check(lib.hmf_adapted_linear_backward(dy.data_ptr(), xp, ldx, exps, t.data_ptr(), weight.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(), ids.data_ptr(),
+                                               M, K, N, r, L, bf16, None if dx is None else dx.data_ptr(), dA.data_ptr(), dB.data_ptr(), ws.data_ptr(), n, st),
+               'hmf_adapted_linear_backward')
     return dx, dA, dB
 
 

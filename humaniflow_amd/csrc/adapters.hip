@@ -6,7 +6,8 @@
 //   u[m] = s_l B_l^T dy[m]                 dx[m] = W^T dy[m] + A_l^T u[m]
 //   dA_l = sum_{m: ids[m] = l} u[m] x[m]^T      dB_l = sum dy[m] t[m]^T     (an adapter without rows: zero)
 //
-// Two forms by the number of rows:
+// Three forms by the number of rows:
+//   one to four (a single image): one launch of dot products.
 //   few rows (M <= kFewRows: a batch of images): the weights are read once and bound everything.  32 x 32 tiles straight from global memory on the fp32 MFMA, the
 //     reduction split over waves and work-groups until the chip is full; the rows' own adapters are dot products of the rows; one joining launch
 //     adds the partial sums (a fixed order), the bias and the adapters' part.  Two launches.
@@ -87,11 +88,11 @@ template <typename T> struct AdArgs {
 // ---------------------------------------------------------------------------------------------------
 // t[m][j] = s_l sum_k x[m][k] A[l][j][k]: one work-group per row, four ranks of a wave at a time, lanes along K
 template <typename T, bool VEC>
-__device__ __forceinline__ void low_row(const AdArgs<T>& a, int m) {
+__device__ __forceinline__ void low_row(const AdArgs<T>& a, int m, float* t) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int l = a.ids[m];
     if (l < 0 || l >= a.L) {                                               // no adapter: zero; an id that no adapter has: NaN, so that it is seen
-        for (int j = threadIdx.x; j < a.r; j += 256) a.t[(long long)m * a.r + j] = l < 0 ? 0.f : nan32();
+        for (int j = threadIdx.x; j < a.r; j += 256) t[j] = l < 0 ? 0.f : nan32();
         return;
     }
     const T* xr = a.x + (long long)m * a.ldx;
@@ -111,7 +112,7 @@ __device__ __forceinline__ void low_row(const AdArgs<T>& a, int m) {
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
             const float v = wave_sum(acc[jj]);
-            if (lane == 0 && j0 + jj < a.r) a.t[(long long)m * a.r + j0 + jj] = s * v;
+            if (lane == 0 && j0 + jj < a.r) t[j0 + jj] = s * v;
         }
     }
 }
@@ -193,11 +194,64 @@ __global__ __launch_bounds__(256) void k_ad_few(const AdArgs<T> a, int tiles_o, 
     __shared__ float red[4 * 32 * 33];
     const int nb = tiles_o * a.ksplit * tiles_m;
     if ((int)blockIdx.x >= nb) {
-        low_row<T, VEC>(a, blockIdx.x - nb);
+        low_row<T, VEC>(a, blockIdx.x - nb, a.t + (long long)(blockIdx.x - nb) * a.r);
         return;
     }
     const int ot = blockIdx.x % tiles_o, rest = blockIdx.x / tiles_o;
     base_tile<T, true, VEC>(a, a.x, a.ldx, a.N, a.K, ot, rest % a.ksplit, rest / a.ksplit, red);
+}
+
+// One to four rows (a single image): everything in ONE launch, since a second one costs as much as the work.  A work-group finds the rows' t itself -- A_l is read once per
+// work-group, from L2 -- and then its waves two outputs each, lanes along K.  1 row, 2,048 -> 1,024, rank 16 in 32 bits: 9 us and two launches in the form below.
+constexpr int kOneRows = 4, kOneBytes = 512 << 10;                          // rows; bytes of A that a work-group reads for them
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void k_ad_one(const AdArgs<T> a) {
+    __shared__ float st[kOneRows][kMaxRank];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n0 = blockIdx.x * 8 + wave * 2;
+    // the outputs' own products first: their loads are on their way while t is found
+    float y[kOneRows][2];
+#pragma unroll
+    for (int m = 0; m < kOneRows; ++m) y[m][0] = y[m][1] = 0.f;
+    const T *w0 = a.w + (long long)min(n0, a.N - 1) * a.K, *w1 = a.w + (long long)min(n0 + 1, a.N - 1) * a.K;
+    for (int k = lane * 4; k < a.K; k += 256) {
+        const f32x4 u0 = load4<VEC>(w0 + k, a.K - k), u1 = load4<VEC>(w1 + k, a.K - k);
+#pragma unroll
+        for (int m = 0; m < kOneRows; ++m)
+            if (m < a.M) {
+                const f32x4 xv = load4<VEC>(a.x + m * a.ldx + k, a.K - k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    y[m][0] = fmaf(xv[e], u0[e], y[m][0]);
+                    y[m][1] = fmaf(xv[e], u1[e], y[m][1]);
+                }
+            }
+    }
+    for (int m = 0; m < a.M; ++m) {
+        low_row<T, VEC>(a, m, st[m]);
+        if (a.t && blockIdx.x == 0) {
+            __syncthreads();
+            for (int j = threadIdx.x; j < a.r; j += 256) a.t[(long long)m * a.r + j] = st[m][j];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < kOneRows; ++m) {
+        if (m >= a.M) break;
+        const int l = a.ids[m];
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            const int n = n0 + o;
+            float v = wave_sum(y[m][o]);
+            float d = 0.f;
+            if (l >= 0 && l < a.L && n < a.N && lane < a.r) d = st[m][lane] * up(a.b[((long long)l * a.N + n) * a.r + lane]);      // r <= 64: a rank per lane
+            v += wave_sum(d);
+            if (lane == 0 && n < a.N) {
+                if (a.bias) v += up(a.bias[n]);
+                down(a.y + (long long)m * a.N + n, l >= a.L ? nan32() : v);
+            }
+        }
+    }
 }
 
 // sum of n values `stride` apart, eight loads in flight (a plain loop waits for every one: 16 splits took 7 us)
@@ -322,14 +376,14 @@ template <typename T> struct Z8<T, true> {
     }
 };
 
-constexpr int kGradLds = 4 * 32 * 64;          // floats
-// T: type of z and of the gradients; ACT8: z is a checkpoint
-template <typename T, bool ACT8>
+constexpr int grad_lds(int waves) { return waves * 32 * 64; }          // floats
+// T: type of z and of the gradients; ACT8: z is a checkpoint; NW: waves of the work-group (4 or 8)
+template <typename T, bool ACT8, int NW>
 __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* rows, int n, int l, long long piece, bool whole, int cb, float* red) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const int c = cb * 128 + 8 * i;
     const bool vec = Z8<T, ACT8>::aligned(g);
-    const int per = ((n + 3) / 4 + 3) & ~3, r0 = wave * per, r1 = min(r0 + per, n);
+    const int per = ((n + NW - 1) / NW + 3) & ~3, r0 = wave * per, r1 = min(r0 + per, n);
     for (int j0 = 0; j0 < r; j0 += 16) {
         const int j = min(j0 + i, r - 1);
         f32x4 acc[8];
@@ -362,12 +416,15 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
         __syncthreads();
         auto total = [&](int t, int e) {
             const int at = (t * 4 + e) * 64 + lane;
-            return ((red[at] + red[at + 32 * 64]) + red[at + 64 * 64]) + red[at + 96 * 64];
-        };
-        if (whole && g.trans) {                                            // wave w: columns c + 2 w, c + 2 w + 1, four ranks each
+            float v = red[at];
 #pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2) {
-                const int t = 2 * wave + t2, jj = j0 + 4 * q;
+            for (int w = 1; w < NW; ++w) v += red[at + w * 32 * 64];
+            return v;
+        };
+        if (whole && g.trans) {                                            // a wave: 8 / NW columns, four ranks each
+#pragma unroll
+            for (int t2 = 0; t2 < 8 / NW; ++t2) {
+                const int t = 8 / NW * wave + t2, jj = j0 + 4 * q;
                 T* po = (T*)g.out + ((long long)l * g.C + c + t) * r + jj;
                 T h[4] __attribute__((aligned(16)));
 #pragma unroll
@@ -385,31 +442,34 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
                     }
                 }
             }
-        } else {                                                           // wave w: rank j0 + 4 q + w, eight columns
-            const int jj = j0 + 4 * q + wave;
-            float v[8];
+        } else {                                                           // a wave: rank j0 + 4 q + (w & 3), TN columns
+            constexpr int TN = 32 / NW;
+            const int e = wave & 3, t0 = (wave >> 2) * TN, jj = j0 + 4 * q + e, c0 = c + t0;
+            float v[TN];
 #pragma unroll
-            for (int t = 0; t < 8; ++t) v[t] = total(t, wave);
+            for (int t = 0; t < TN; ++t) v[t] = total(t0 + t, e);
             if (jj < r) {
                 if (!whole) {
-                    float* po = g.part + (piece * r + jj) * g.C + c;
+                    float* po = g.part + (piece * r + jj) * g.C + c0;
 #pragma unroll
-                    for (int t = 0; t < 8; ++t)
-                        if (c + t < g.C) po[t] = v[t];
+                    for (int t = 0; t < TN; ++t)
+                        if (c0 + t < g.C) po[t] = v[t];
                 } else {
-                    T* po = (T*)g.out + ((long long)l * r + jj) * g.C + c;
-                    T h[8] __attribute__((aligned(16)));
+                    T* po = (T*)g.out + ((long long)l * r + jj) * g.C + c0;
+                    T h[TN] __attribute__((aligned(16)));
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) down(h + t, v[t]);
+                    for (int t = 0; t < TN; ++t) down(h + t, v[t]);
                     if (g.C % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {
-                        if (c < g.C) {
-                            *(uint4*)po = *(const uint4*)h;
-                            if (sizeof(T) == 4) *((uint4*)po + 1) = *((const uint4*)h + 1);
+                        if (c0 < g.C) {
+                            if (sizeof(h) == 8) *(uint2*)po = *(const uint2*)h;
+                            else
+#pragma unroll
+                                for (int k = 0; k < (int)sizeof(h) / 16; ++k) *((uint4*)po + k) = *((const uint4*)h + k);
                         }
                     } else {
 #pragma unroll
-                        for (int t = 0; t < 8; ++t)
-                            if (c + t < g.C) po[t] = h[t];
+                        for (int t = 0; t < TN; ++t)
+                            if (c0 + t < g.C) po[t] = h[t];
                     }
                 }
             }
@@ -435,7 +495,7 @@ __device__ __forceinline__ int rows_of(const int* ids, int M, int l, int* rows, 
 // few rows, backward, first launch: dx's partial sums, u, dB
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_ad_few_back(const AdArgs<T> a, const AdGrad db, int tiles_o, int tiles_m) {
-    __shared__ float red[kGradLds];
+    __shared__ float red[grad_lds(4)];
     __shared__ int rows[kFewRows], cnt[4];
     const int nb = a.dx ? tiles_o * a.ksplit * tiles_m : 0;
     int id = blockIdx.x;
@@ -452,13 +512,13 @@ __global__ __launch_bounds__(256) void k_ad_few_back(const AdArgs<T> a, const Ad
     id -= a.M;
     const int l = id / db.blocks;
     const int n = rows_of(a.ids, a.M, l, rows, cnt);
-    grad_piece<T, false>(db, a.r, rows, n, l, 0, true, id - l * db.blocks, red);
+    grad_piece<T, false, 4>(db, a.r, rows, n, l, 0, true, id - l * db.blocks, red);
 }
 
 // second launch: dx = partial sums + A_l^T u, dA
 template <typename T, bool ACT8>
 __global__ __launch_bounds__(256) void k_ad_few_back2(const AdArgs<T> a, const AdGrad da, int join_wgs) {
-    __shared__ float red[kGradLds];
+    __shared__ float red[grad_lds(4)];
     __shared__ int rows[kFewRows], cnt[4];
     int id = blockIdx.x;
     if (id < join_wgs) {
@@ -475,7 +535,7 @@ __global__ __launch_bounds__(256) void k_ad_few_back2(const AdArgs<T> a, const A
     id -= join_wgs;
     const int l = id / da.blocks;
     const int n = rows_of(a.ids, a.M, l, rows, cnt);
-    grad_piece<T, ACT8>(da, a.r, rows, n, l, 0, true, id - l * da.blocks, red);
+    grad_piece<T, ACT8, 4>(da, a.r, rows, n, l, 0, true, id - l * da.blocks, red);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -620,15 +680,15 @@ template <> struct Mma<bf16_t> {
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ bool finite(bf16_t v) { return (v & 0x7f80u) != 0x7f80u; }
 
-// Piece z of the order: segment l (of n) has max(MIN, ceil(rows / R)) pieces of R rows, one behind the other.  All lanes of a wave return the same: the segment, which of
-// its pieces this is, how many it has; l = n: no such piece.
+// Piece z of the order: segment l (of n) has max(MIN, ceil(rows / R)) pieces of R rows, one behind the other.  All lanes of a wave return the same: the segment, how many
+// pieces it has, this one's first place and its end; l = n: no such piece.
 template <int R, int MIN>
-__device__ __forceinline__ void find_piece(const int* seg, int n, int z, int& l, int& p, int& np) {
+__device__ __forceinline__ void find_piece(const int* seg, int n, int z, int& l, int& np, int& at, int& end) {
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int l0 = 0; l0 < n; l0 += 64) {
         const int li = l0 + lane;
-        const int rows = li < n ? seg[li + 1] - seg[li] : 0;
+        const int s0 = seg[min(li, n)], s1 = seg[min(li + 1, n)], rows = s1 - s0;
         const int mine = li < n ? max(MIN, (rows + R - 1) / R) : 0;
         int incl = mine;
 #pragma unroll
@@ -641,13 +701,14 @@ __device__ __forceinline__ void find_piece(const int* seg, int n, int z, int& l,
             const int k = __ffsll((long long)over) - 1;
             l = l0 + k;
             np = __shfl(mine, k);
-            p = z - (base + __shfl(incl, k) - np);
+            at = __shfl(s0, k) + (z - (base + __shfl(incl, k) - np)) * R;
+            end = min(at + R, __shfl(s1, k));
             return;
         }
         base += __shfl(incl, 63);
     }
     l = n;
-    p = np = 0;
+    np = at = end = 0;
 }
 
 typedef __attribute__((address_space(3))) void* ad_lds_t;
@@ -676,13 +737,12 @@ __global__ __launch_bounds__(1024) void k_ad_low(const AdLow a) {
     __shared__ __attribute__((aligned(16))) char smem[16 * 2 * U * 1024];
     float* red = (float*)smem;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, q = lane >> 4;
-    int ad, pc, np;
-    find_piece<16, 0>(a.seg, a.L + 1, blockIdx.x, ad, pc, np);              // the rows without an adapter are the last segment
+    int ad, np, first, end;
+    find_piece<16, 0>(a.seg, a.L + 1, blockIdx.x, ad, np, first, end);      // the rows without an adapter are the last segment
     if (ad > a.L) return;
     ad = __builtin_amdgcn_readfirstlane(ad);
-    const int end = a.seg[ad + 1], at = a.seg[ad] + 16 * pc + i;
-    const bool live = at < end;
-    const int p = min(at, end - 1), m = a.order[p];                         // places past the segment's last row repeat it and write nothing
+    const bool live = first + i < end;
+    const int p = min(first + i, end - 1), m = a.order[p];                         // places past the segment's last row repeat it and write nothing
     if (ad == a.L) {                                                        // no adapter: zero; an id that no adapter has: NaN
         if (live && q == 0)
             for (int j = wave; j < a.r; j += 16) a.low[(long long)m * a.r + j] = a.key[p] < 0 ? 0.f : nan32();
@@ -825,7 +885,20 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
             const bool mine = live && slot[row] == ad;
             const float* pl = a.low + (long long)(mine ? rowid[row] : 0) * a.r + j0;
 #pragma unroll
-            for (int k = 0; k < E; ++k) ex[s][k] = (mine && j0 + k < a.r) ? pl[k] : 0.f;
+            for (int k = 0; k < E; ++k) ex[s][k] = 0.f;
+            if (a.r % 4 == 0) {
+#pragma unroll
+                for (int k = 0; k < E; k += 4)
+                    if (mine && j0 + k < a.r) {
+                        const f32x4 u = *(const f32x4*)(pl + k);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) ex[s][k + e] = u[e];
+                    }
+            } else if (mine) {
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (j0 + k < a.r) ex[s][k] = pl[k];
+            }
             if (vec_v) {
 #pragma unroll
                 for (int k = 0; k < E; ++k) ew[s][k] = 0;
@@ -883,10 +956,10 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
 #pragma unroll
             for (int v = 0; v < NT; ++v) acc[t][v] = X::mma32(fw[g & 1][t], fx[g & 1][v], acc[t][v]);
     };
-    if (ne > 0) fetch(0);
 #pragma unroll
     for (int c = 0; c < S - 1; ++c)
         if (c < kc) issue(c, 0, ND);
+    if (ne > 0) fetch(0);                                                   // behind the first requests: the counts waited for below are then only stricter than they say
     // One chunk: its own fragments group by group, each read under the MFMAs of the group before; chunk c + 1 is there too (at most the one behind it is on its way),
     // so the next chunk's first fragments are read under this one's last MFMAs and the matrix pipe does not drain at the barrier.
     auto iteration = [&](int c, auto MORE) {
@@ -1017,18 +1090,18 @@ __global__ __launch_bounds__(256) void k_ad_sum(const float* __restrict__ partia
 }
 
 template <typename T, bool ACT8>
-__global__ __launch_bounds__(256) void k_ad_grads(const AdGrad da, const AdGrad db, const int* __restrict__ order, const int* __restrict__ seg, int r, int L) {
-    __shared__ float red[kGradLds];
+__global__ __launch_bounds__(512) void k_ad_grads(const AdGrad da, const AdGrad db, const int* __restrict__ order, const int* __restrict__ seg, int r, int L) {
+    __shared__ float red[grad_lds(8)];
     __shared__ int rows[kFewRows];
-    int l, p, np;
-    find_piece<kFewRows, 1>(seg, L, blockIdx.y, l, p, np);
+    int l, np, s0, end;
+    find_piece<kFewRows, 1>(seg, L, blockIdx.y, l, np, s0, end);
     if (l >= L) return;
-    const int s0 = seg[l] + p * kFewRows, n = min(kFewRows, seg[l + 1] - s0);
+    const int n = end - s0;
     if ((int)threadIdx.x < n) rows[threadIdx.x] = order[s0 + threadIdx.x];
     __syncthreads();
     const int cb = blockIdx.x;
-    if (cb < da.blocks) grad_piece<T, ACT8>(da, r, rows, n, l, blockIdx.y, np == 1, cb, red);
-    else grad_piece<T, false>(db, r, rows, n, l, blockIdx.y, np == 1, cb - da.blocks, red);
+    if (cb < da.blocks) grad_piece<T, ACT8, 8>(da, r, rows, n, l, blockIdx.y, np == 1, cb, red);
+    else grad_piece<T, false, 8>(db, r, rows, n, l, blockIdx.y, np == 1, cb - da.blocks, red);
 }
 
 // sums of the adapters that had several pieces, in the pieces' order; a column of work-groups per adapter, gone at once where there is nothing to add
@@ -1189,6 +1262,13 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
     const int V = 16 / (int)sizeof(T);
     const bool vec = K % V == 0 && ldx % V == 0 && !off16(x) && !off16(w) && !off16(a);
+    if (M <= kOneRows && (long long)M * r * K * (int)sizeof(T) <= kOneBytes) {
+        g.t = t;
+        if (vec) hipLaunchKernelGGL((k_ad_one<T, true>), dim3(blocks_of(N, 8)), dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((k_ad_one<T, false>), dim3(blocks_of(N, 8)), dim3(256), 0, st, g);
+        HMF_LAUNCH_CHECK();
+        return HMF_OK;
+    }
     if (M <= kFewRows) {
         few_split(M, N, K, &g.ksplit, &g.kw);
         g.partial = (float*)(ws + o.partial);
@@ -1283,8 +1363,8 @@ static int backward_t(const T* dy, const void* x, long long ldx, const unsigned 
     ga.part = (float*)(ws + o.part_a);
     gb.part = (float*)(ws + o.part_b);
     const dim3 grid(ga.blocks + gb.blocks, L + M / kFewRows);
-    if (exps) hipLaunchKernelGGL((k_ad_grads<T, true>), grid, dim3(256), 0, st, ga, gb, order, seg, r, L);
-    else hipLaunchKernelGGL((k_ad_grads<T, false>), grid, dim3(256), 0, st, ga, gb, order, seg, r, L);
+    if (exps) hipLaunchKernelGGL((k_ad_grads<T, true>), grid, dim3(512), 0, st, ga, gb, order, seg, r, L);
+    else hipLaunchKernelGGL((k_ad_grads<T, false>), grid, dim3(512), 0, st, ga, gb, order, seg, r, L);
     HMF_LAUNCH_CHECK();
     hipLaunchKernelGGL(k_ad_grad_join<T>, dim3(std::min(256, blocks_of((long long)r * (K + N), 256)), L), dim3(256), 0, st, ga, gb, seg, r, L);
     HMF_LAUNCH_CHECK();
