@@ -131,7 +131,18 @@ __device__ __forceinline__ void up_row(const AdArgs<T>& a, int m, float* red) {
     const T* bl = a.b + (long long)l * a.N * a.r;
     float acc = 0.f;
     if (g < per)
-        for (int n = wave * per + g; n < a.N; n += 4 * per) acc = fmaf(up(dr[n]), up(bl[(long long)n * a.r + j]), acc);
+        for (int nb = wave * per + g; nb < a.N; nb += 4 * per * 16) {      // 16 rows of B in flight (one: 1,378 outputs at rank 63 took 54 us)
+            T d[16], b[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int n = min(nb + 4 * per * k, a.N - 1);
+                d[k] = dr[n];
+                b[k] = bl[(long long)n * a.r + j];
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (nb + 4 * per * k < a.N) acc = fmaf(up(d[k]), up(b[k]), acc);
+        }
     red[wave * 64 + lane] = acc;
     __syncthreads();
     if (threadIdx.x < a.r) {
@@ -300,7 +311,7 @@ __global__ __launch_bounds__(64) void k_ad_join(const AdArgs<T> a) {
 
 // ---------------------------------------------------------------------------------------------------
 // gradients of the adapters: G[j][c] = sum over an adapter's rows of p[m][j] z[m][c], p (M, r) in 32 bits;  dA: p = u, z = x (or its 8-bit checkpoint);  dB^T: p = t, z = dy.
-// A work-group owns (adapter, piece of <= 256 of its rows, 128 columns); its waves take a quarter of the rows each, 4 rows per 16 x 16 x 4 MFMA step, and every lane the
+// A work-group owns (adapter, piece of <= 256 of its rows, 128 columns, 16 ranks); its waves take a part of the rows each, 4 rows per 16 x 16 x 4 MFMA step, and every lane the
 // eight columns 8 i .. 8 i + 7 (one load of 8 to 32 bytes feeds eight MFMA tiles); they meet in LDS in a fixed order.  More pieces than one: partial sums in the
 // workspace, joined by k_ad_grad_join.  Tiles of 32 ranks (32 x 32 x 2) waste half the matrix work at the usual ranks of up to 16.
 // ---------------------------------------------------------------------------------------------------
@@ -311,14 +322,14 @@ struct AdGrad {
     void* out;                         // (L, r, C), or (L, C, r) with trans
     float* part;                       // [pieces][r][C]
     long long ldz;
-    int C, trans, blocks;              // blocks: column blocks of 128
+    int C, Cp, trans, blocks;          // columns, columns that may be read; blocks: blocks of 128 columns x 16 ranks, columns first
 };
 
 // eight consecutive elements of a row of z, as they lie in memory; columns past C read as zero
 template <typename T, bool ACT8> struct Z8;
 template <> struct Z8<float, false> {
     f32x4 d[2];
-    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.ldz % 4 == 0 && g.C % 8 == 0 && ((uintptr_t)g.z & 15) == 0; }
+    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.ldz % 4 == 0 && g.Cp % 8 == 0 && ((uintptr_t)g.z & 15) == 0; }
     __device__ __forceinline__ void load(const AdGrad& g, int m, int c, bool vec) {
         const float* p = (const float*)g.z + (long long)m * g.ldz + c;
         if (vec) {
@@ -334,7 +345,7 @@ template <> struct Z8<float, false> {
 };
 template <> struct Z8<bf16_t, false> {
     u16x8 d;
-    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.ldz % 8 == 0 && g.C % 8 == 0 && ((uintptr_t)g.z & 15) == 0; }
+    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.ldz % 8 == 0 && g.Cp % 8 == 0 && ((uintptr_t)g.z & 15) == 0; }
     __device__ __forceinline__ void load(const AdGrad& g, int m, int c, bool vec) {
         const bf16_t* p = (const bf16_t*)g.z + (long long)m * g.ldz + c;
         if (vec) {
@@ -379,98 +390,104 @@ template <typename T> struct Z8<T, true> {
 constexpr int grad_lds(int waves) { return waves * 32 * 64; }          // floats
 // T: type of z and of the gradients; ACT8: z is a checkpoint; NW: waves of the work-group (4 or 8)
 template <typename T, bool ACT8, int NW>
-__device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* rows, int n, int l, long long piece, bool whole, int cb, float* red) {
+__device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* rows, int n, int l, long long piece, bool whole, int block, float* red) {
+    const int ncb = (g.C + 127) / 128, cb = block % ncb, j0 = block / ncb * 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const int c = cb * 128 + 8 * i;
+    if (n == 0) {                                                          // an adapter without rows has one piece: its part of the result is zero
+        const int c0 = cb * 128, w = min(128, g.C - c0), nj = min(16, r - j0);
+        for (int e = threadIdx.x; e < 128 * 16; e += NW * 64) {
+            const int jj = g.trans ? e & 15 : e >> 7, cc = g.trans ? e >> 4 : e & 127;      // along what lies next to each other
+            if (jj < nj && cc < w) down((T*)g.out + (g.trans ? ((long long)l * g.C + c0 + cc) * r + j0 + jj : ((long long)l * r + j0 + jj) * g.C + c0 + cc), 0.f);
+        }
+        return;
+    }
     const bool vec = Z8<T, ACT8>::aligned(g);
     const int per = ((n + NW - 1) / NW + 3) & ~3, r0 = wave * per, r1 = min(r0 + per, n);
-    for (int j0 = 0; j0 < r; j0 += 16) {
-        const int j = min(j0 + i, r - 1);
-        f32x4 acc[8];
+    const int j = min(j0 + i, r - 1);
+    f32x4 acc[8];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        constexpr int U = 8;
-        for (int rr = r0; rr < r1; rr += 4 * U) {
-            Z8<T, ACT8> z[U];
-            float pv[U];
+    for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 8;
+    for (int rr = r0; rr < r1; rr += 4 * U) {
+        Z8<T, ACT8> z[U];
+        float pv[U];
 #pragma unroll
-            for (int s = 0; s < U; ++s) {
-                const int at = rr + 4 * s + q;
-                const bool in = at < r1;
-                const int m = rows[in ? at : 0];
-                pv[s] = (in && j0 + i < r) ? g.p[(long long)m * r + j] : 0.f;
-                z[s].zero();
-                if (in) z[s].load(g, m, c, vec);
-            }
-#pragma unroll
-            for (int s = 0; s < U; ++s)
-#pragma unroll
-                for (int t = 0; t < 8; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[s], z[s].get(t), acc[t], 0, 0, 0);
+        for (int s = 0; s < U; ++s) {
+            const int at = rr + 4 * s + q;
+            const bool in = at < r1;
+            const int m = rows[in ? at : 0];
+            pv[s] = (in && j0 + i < r) ? g.p[(long long)m * r + j] : 0.f;
+            z[s].zero();
+            if (in) z[s].load(g, m, c, vec);
         }
-        // element e of tile t: rank j0 + 4 q + e of column c + t
-        __syncthreads();
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
+        for (int s = 0; s < U; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) red[(wave * 32 + t * 4 + e) * 64 + lane] = acc[t][e];
-        __syncthreads();
-        auto total = [&](int t, int e) {
-            const int at = (t * 4 + e) * 64 + lane;
-            float v = red[at];
+            for (int t = 0; t < 8; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[s], z[s].get(t), acc[t], 0, 0, 0);
+    }
+    // element e of tile t: rank j0 + 4 q + e of column c + t
 #pragma unroll
-            for (int w = 1; w < NW; ++w) v += red[at + w * 32 * 64];
-            return v;
-        };
-        if (whole && g.trans) {                                            // a wave: 8 / NW columns, four ranks each
+    for (int t = 0; t < 8; ++t)
 #pragma unroll
-            for (int t2 = 0; t2 < 8 / NW; ++t2) {
-                const int t = 8 / NW * wave + t2, jj = j0 + 4 * q;
-                T* po = (T*)g.out + ((long long)l * g.C + c + t) * r + jj;
-                T h[4] __attribute__((aligned(16)));
+        for (int e = 0; e < 4; ++e) red[(wave * 32 + t * 4 + e) * 64 + lane] = acc[t][e];
+    __syncthreads();
+    auto total = [&](int t, int e) {
+        const int at = (t * 4 + e) * 64 + lane;
+        float v = red[at];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) down(h + e, total(t, e));
-                if (c + t < g.C) {
-                    if (r % 4 == 0 && ((uintptr_t)g.out & (4 * sizeof(T) - 1)) == 0) {
-                        if (jj < r) {
-                            if (sizeof(T) == 4) *(uint4*)po = *(const uint4*)h;
-                            else *(uint2*)po = *(const uint2*)h;
-                        }
-                    } else {
+        for (int w = 1; w < NW; ++w) v += red[at + w * 32 * 64];
+        return v;
+    };
+    if (whole && g.trans) {                                            // a wave: 8 / NW columns, four ranks each
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (jj + e < r) po[e] = h[e];
+        for (int t2 = 0; t2 < 8 / NW; ++t2) {
+            const int t = 8 / NW * wave + t2, jj = j0 + 4 * q;
+            T* po = (T*)g.out + ((long long)l * g.C + c + t) * r + jj;
+            T h[4] __attribute__((aligned(16)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) down(h + e, total(t, e));
+            if (c + t < g.C) {
+                if (r % 4 == 0 && ((uintptr_t)g.out & (4 * sizeof(T) - 1)) == 0) {
+                    if (jj < r) {
+                        if (sizeof(T) == 4) *(uint4*)po = *(const uint4*)h;
+                        else *(uint2*)po = *(const uint2*)h;
                     }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (jj + e < r) po[e] = h[e];
                 }
             }
-        } else {                                                           // a wave: rank j0 + 4 q + (w & 3), TN columns
-            constexpr int TN = 32 / NW;
-            const int e = wave & 3, t0 = (wave >> 2) * TN, jj = j0 + 4 * q + e, c0 = c + t0;
-            float v[TN];
+        }
+    } else {                                                           // a wave: rank j0 + 4 q + (w & 3), TN columns
+        constexpr int TN = 32 / NW;
+        const int e = wave & 3, t0 = (wave >> 2) * TN, jj = j0 + 4 * q + e, c0 = c + t0;
+        float v[TN];
 #pragma unroll
-            for (int t = 0; t < TN; ++t) v[t] = total(t0 + t, e);
-            if (jj < r) {
-                if (!whole) {
-                    float* po = g.part + (piece * r + jj) * g.C + c0;
+        for (int t = 0; t < TN; ++t) v[t] = total(t0 + t, e);
+        if (jj < r) {
+            if (!whole) {
+                float* po = g.part + (piece * r + jj) * g.C + c0;
+#pragma unroll
+                for (int t = 0; t < TN; ++t)
+                    if (c0 + t < g.C) po[t] = v[t];
+            } else {
+                T* po = (T*)g.out + ((long long)l * r + jj) * g.C + c0;
+                T h[TN] __attribute__((aligned(16)));
+#pragma unroll
+                for (int t = 0; t < TN; ++t) down(h + t, v[t]);
+                if (g.C % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {
+                    if (c0 < g.C) {
+                        if (sizeof(h) == 8) *(uint2*)po = *(const uint2*)h;
+                        else
+#pragma unroll
+                            for (int k = 0; k < (int)sizeof(h) / 16; ++k) *((uint4*)po + k) = *((const uint4*)h + k);
+                    }
+                } else {
 #pragma unroll
                     for (int t = 0; t < TN; ++t)
-                        if (c0 + t < g.C) po[t] = v[t];
-                } else {
-                    T* po = (T*)g.out + ((long long)l * r + jj) * g.C + c0;
-                    T h[TN] __attribute__((aligned(16)));
-#pragma unroll
-                    for (int t = 0; t < TN; ++t) down(h + t, v[t]);
-                    if (g.C % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {
-                        if (c0 < g.C) {
-                            if (sizeof(h) == 8) *(uint2*)po = *(const uint2*)h;
-                            else
-#pragma unroll
-                                for (int k = 0; k < (int)sizeof(h) / 16; ++k) *((uint4*)po + k) = *((const uint4*)h + k);
-                        }
-                    } else {
-#pragma unroll
-                        for (int t = 0; t < TN; ++t)
-                            if (c0 + t < g.C) po[t] = h[t];
-                    }
+                        if (c0 + t < g.C) po[t] = h[t];
                 }
             }
         }
@@ -545,7 +562,7 @@ __global__ __launch_bounds__(256) void k_ad_few_back2(const AdArgs<T> a, const A
 //   order: the rows by adapter (those without one last), each adapter's in their own order; key: their ids in that order;  seg[l]: where adapter l begins (seg[L]:
 //     rows without, seg[L + 1] = M).  Work-group l counts the rows in front of its own adapter's, then places these: its sixteen waves take a range of the rows
 //     each, nothing is shared between work-groups.
-//   Copies: dst[b][r][c] (pitch ldd, columns past C zero) = src[b][r][c] or, transposed, src[b][c][r]: 64 x 64 tiles, through LDS.
+//   Copies: dst[b][r][c] (pitch ldd, columns past C zero) = src[b][r][c] or, transposed, src[b][c][r], through LDS.
 struct AdCopy {
     const void* src;
     void* dst;
@@ -562,7 +579,7 @@ struct AdPrep {
 constexpr int kPrep = 1024;                // threads: the plan of some thousand rows is two rounds of loads, not thirty
 template <typename T>
 __global__ __launch_bounds__(kPrep) void k_ad_prep(const AdPrep a) {
-    __shared__ T s[64][65];
+    __shared__ T s[64][257];
     __shared__ int cnt[32];
     int id = blockIdx.x;
     if (id <= a.L) {
@@ -620,28 +637,30 @@ __global__ __launch_bounds__(kPrep) void k_ad_prep(const AdPrep a) {
     while (k < a.ncopy && id >= a.copy[k].tiles) id -= a.copy[k++].tiles;
     if (k >= a.ncopy) return;
     const AdCopy& c = a.copy[k];
-    const int bt = id / (c.tr * c.tc), rest = id - bt * c.tr * c.tc, r0 = rest / c.tc * 64, c0 = rest % c.tc * 64;
+    const int bt = id / (c.tr * c.tc), rest = id - bt * c.tr * c.tc, ir = rest / c.tc, ic = rest - ir * c.tc;
     const T* src = (const T*)c.src + bt * c.sbs;
     T* dst = (T*)c.dst + bt * c.dbs;
     const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    T v[4];
+    T v[16];                                                                // sixteen elements of a thread in flight
+    if (!c.trans) {                                                         // 256 rows x 64 columns
+        const int r0 = ir * 256 + y, cc = ic * 64 + x;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int rr = c.trans ? r0 + x : r0 + y + 16 * j, cc = c.trans ? c0 + y + 16 * j : c0 + x;
-        v[j] = (rr < c.R && cc < c.C) ? src[c.trans ? (long long)cc * c.lds_ + rr : (long long)rr * c.lds_ + cc] : (T)0;
-    }
-    if (!c.trans) {                                                        // uniform
+        for (int j = 0; j < 16; ++j) v[j] = (r0 + 16 * j < c.R && cc < c.C) ? src[(long long)(r0 + 16 * j) * c.lds_ + cc] : (T)0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (r0 + y + 16 * j < c.R && c0 + x < c.Cp) dst[(long long)(r0 + y + 16 * j) * c.ldd + c0 + x] = v[j];
+        for (int j = 0; j < 16; ++j)
+            if (r0 + 16 * j < c.R && cc < c.Cp) dst[(long long)(r0 + 16 * j) * c.ldd + cc] = v[j];
         return;
     }
+    const int r0 = ir * 64, c0 = ic * 256;                                  // 64 rows x 256 columns of the destination
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[x][y + 16 * j] = v[j];
+    for (int j = 0; j < 16; ++j) v[j] = (r0 + x < c.R && c0 + y + 16 * j < c.C) ? src[(long long)(c0 + y + 16 * j) * c.lds_ + r0 + x] : (T)0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[x][y + 16 * j] = v[j];
     __syncthreads();
+    const int xc = threadIdx.x & 255, yr = threadIdx.x >> 8;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (r0 + y + 16 * j < c.R && c0 + x < c.Cp) dst[(long long)(r0 + y + 16 * j) * c.ldd + c0 + x] = s[y + 16 * j][x];
+    for (int j = 0; j < 16; ++j)
+        if (r0 + yr + 4 * j < c.R && c0 + xc < c.Cp) dst[(long long)(r0 + yr + 4 * j) * c.ldd + c0 + xc] = s[yr + 4 * j][xc];
 }
 
 // What the two types differ in.  A chunk of the reduction is 128 bytes of a row (BK elements) in both, a fragment 16 bytes.
@@ -1224,7 +1243,7 @@ static int check_sizes(const char* who, int M, int K, int N, int r, int L) {
 }
 
 static AdCopy copy_job(const void* src, void* dst, long long lds_, long long ldd, long long sbs, long long dbs, int batches, int R, int C, int Cp, int trans) {
-    AdCopy c{src, dst, lds_, ldd, sbs, dbs, R, C, Cp, trans, 0, blocks_of(R, 64), blocks_of(Cp, 64)};
+    AdCopy c{src, dst, lds_, ldd, sbs, dbs, R, C, Cp, trans, 0, blocks_of(R, trans ? 64 : 256), blocks_of(Cp, trans ? 256 : 64)};
     c.tiles = batches * c.tr * c.tc;
     return c;
 }
@@ -1318,8 +1337,8 @@ static int backward_t(const T* dy, const void* x, long long ldx, const unsigned 
     g.dy = dy; g.w = w; g.a = a; g.b = b; g.scale = scale; g.ids = ids; g.dx = dx; g.u = (float*)(ws + o.u);
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
     AdGrad ga{}, gb{};
-    ga.p = g.u; ga.z = x; ga.exps = exps; ga.out = da; ga.ldz = ldx; ga.C = K; ga.trans = 0; ga.blocks = blocks_of(K, 128);
-    gb.p = t; gb.z = dy; gb.out = db; gb.ldz = N; gb.C = N; gb.trans = 1; gb.blocks = blocks_of(N, 128);
+    ga.p = g.u; ga.z = x; ga.exps = exps; ga.out = da; ga.ldz = ldx; ga.C = ga.Cp = K; ga.trans = 0; ga.blocks = blocks_of(K, 128) * blocks_of(r, 16);
+    gb.p = t; gb.z = dy; gb.out = db; gb.ldz = N; gb.C = gb.Cp = N; gb.trans = 1; gb.blocks = blocks_of(N, 128) * blocks_of(r, 16);
     const int V = 16 / (int)sizeof(T);
     const bool vec = N % V == 0 && !off16(dy);
     if (M <= kFewRows) {
@@ -1347,6 +1366,7 @@ static int backward_t(const T* dy, const void* x, long long ldx, const unsigned 
     if (N != Np) {
         pr.copy[pr.ncopy++] = copy_job(dy, ws + o.dyp, N, Np, 0, 0, 1, M, N, Np, 0);
         dyp = (const T*)(ws + o.dyp);
+        gb.z = dyp; gb.ldz = Np; gb.Cp = Np;                               // the padded rows serve dB's aligned loads too
     }
     if (int rc = prepare<T>(pr, st)) return rc;
     AdLow lo{};
