@@ -663,17 +663,13 @@ __global__ __launch_bounds__(kPrep) void k_ad_prep(const AdPrep a) {
         if (r0 + yr + 4 * j < c.R && c0 + xc < c.Cp) dst[(long long)(r0 + yr + 4 * j) * c.ldd + c0 + xc] = s[yr + 4 * j][xc];
 }
 
-// What the two types differ in.  A chunk of the reduction is 128 bytes of a row (BK elements) in both, a fragment 16 bytes.
+// What the two types differ in.  A fragment is 16 bytes of a row in both.
 template <typename T> struct Mma;
 template <> struct Mma<float> {
-    static constexpr int BK = 32, E = 4, HL = 1;                            // E: elements of 16 bytes; HL: columns of the reduction per rank
+    static constexpr int E = 4, HL = 1, STEPS = 4;                          // elements of 16 bytes; columns of the reduction per rank; MFMA steps of 32 bytes
     typedef f32x4 frag;
     // 32 bytes of both operands' rows: 4 steps of the 32 x 32 x 2 MFMA, lane half q holds elements 4 q .. 4 q + 3
-    static __device__ __forceinline__ f32x16 mma32(frag a, frag b, f32x16 c) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-        return c;
-    }
+    static __device__ __forceinline__ f32x16 mma32(frag a, frag b, f32x16 c, int e) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0); }
     // 64 bytes: 4 steps of the 16 x 16 x 4 MFMA, lane quarter holds its 16 bytes
     static __device__ __forceinline__ f32x4 mma16(frag a, frag b, f32x4 c) {
 #pragma unroll
@@ -683,9 +679,9 @@ template <> struct Mma<float> {
     static __device__ __forceinline__ float part(float v, int) { return v; }
 };
 template <> struct Mma<bf16_t> {
-    static constexpr int BK = 64, E = 8, HL = 2;
+    static constexpr int E = 8, HL = 2, STEPS = 1;
     typedef u16x8 frag;
-    static __device__ __forceinline__ f32x16 mma32(frag a, frag b, f32x16 c) {
+    static __device__ __forceinline__ f32x16 mma32(frag a, frag b, f32x16 c, int) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ f32x4 mma16(frag a, frag b, f32x4 c) {
@@ -969,11 +965,13 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
             fx[g & 1][t] = *(const frag*)(px + st * STAGE + go[g] + t * 32 * RB);
         }
     };
-    auto mma = [&](int g) {
+    auto mma = [&](int g) {                                                 // step by step over the tiles: the next MFMA is never the one that waits for the last
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int e = 0; e < X::STEPS; ++e)
 #pragma unroll
-            for (int v = 0; v < NT; ++v) acc[t][v] = X::mma32(fw[g & 1][t], fx[g & 1][v], acc[t][v]);
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int v = 0; v < NT; ++v) acc[t][v] = X::mma32(fw[g & 1][t], fx[g & 1][v], acc[t][v], e);
     };
 #pragma unroll
     for (int c = 0; c < S - 1; ++c)
@@ -988,7 +986,7 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const int st = c & (S - 1);
-        constexpr int nm = NT * NT * (sizeof(T) == 4 ? 4 : 1);
+        constexpr int nm = NT * NT * X::STEPS;
         auto group = [&](auto index) {
             constexpr int g = decltype(index)::value;
             if (g + 1 < G) frags(st, g + 1);
@@ -1172,7 +1170,7 @@ static void gemm_shape(int M, int O, int Cp, size_t z, int* bt, int* rb, int* sp
     *bt = big >= 192 ? 128 : 64;
     *rb = big > 256 && z == 2 ? 64 : 128;
     const int kc = (int)(Cp * z / *rb), tiles = blocks_of(M, *bt) * blocks_of(O, *bt);
-    const int want = tiles >= 256 ? 1 : std::max(1, std::min(kc / (z == 4 ? 8 : 16), 512 / tiles));
+    const int want = tiles >= 256 || *bt == 128 ? 1 : std::max(1, std::min(kc / (z == 4 ? 8 : 16), 512 / tiles));
     *per = blocks_of(kc, want);
     *splits = blocks_of(kc, *per);
 }
