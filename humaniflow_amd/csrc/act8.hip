@@ -60,12 +60,7 @@ __device__ __forceinline__ unsigned int max_over_quarters(unsigned int m) {
     return max(m, (unsigned)__shfl_xor((int)m, 32));
 }
 __device__ __forceinline__ float bf16_to_f32(unsigned short h) { return __uint_as_float((unsigned)h << 16); }
-// round to nearest even; a NaN keeps its sign and stays one
-__device__ __forceinline__ unsigned short f32_to_bf16(float f) {
-    const unsigned int u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)((u >> 16) | 0x40u);
-    return (unsigned short)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
+__device__ __forceinline__ unsigned short f32_to_bf16(float f) { return __builtin_bit_cast(unsigned short, (__bf16)f); }      // nearest even
 
 // NT: past the caches.  A map of more than half the Infinity Cache (256 MB) is gone from it before its reader comes, and only pushes out what the next kernels
 // read: the backward of 294,912 x 256 takes 247 us with, 269 us without; a small map's reader finds it there.  (The forward's map: 202 us without, 207 us with.)

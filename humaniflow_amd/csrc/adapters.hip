@@ -31,11 +31,7 @@ constexpr int kMaxRank = 64;
 
 __device__ __forceinline__ float up(float v) { return v; }
 __device__ __forceinline__ float up(bf16_t h) { return __uint_as_float((unsigned)h << 16); }
-__device__ __forceinline__ bf16_t to_bf16(float f) {                       // nearest even, a NaN stays one
-    const unsigned int u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (bf16_t)((u >> 16) | 0x40u);
-    return (bf16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
+__device__ __forceinline__ bf16_t to_bf16(float f) { return __builtin_bit_cast(bf16_t, (__bf16)f); }      // nearest even, one instruction (a NaN stays one)
 __device__ __forceinline__ void down(float* p, float v) { *p = v; }
 __device__ __forceinline__ void down(bf16_t* p, float v) { *p = to_bf16(v); }
 
@@ -316,12 +312,12 @@ __global__ __launch_bounds__(64) void k_ad_join(const AdArgs<T> a) {
 // workspace, joined by k_ad_grad_join.  Tiles of 32 ranks (32 x 32 x 2) waste half the matrix work at the usual ranks of up to 16.
 // ---------------------------------------------------------------------------------------------------
 struct AdGrad {
-    const float* p;
+    const float* p;                    // pitch ldp
     const void* z;                     // rows of pitch ldz, or the codes (M, C)
     const unsigned char* exps;         // with codes
     void* out;                         // (L, r, C), or (L, C, r) with trans
     float* part;                       // [pieces][r][C]
-    long long ldz;
+    long long ldz, ldp;
     int C, Cp, trans, blocks;          // columns, columns that may be read; blocks: blocks of 128 columns x 16 ranks, columns first
 };
 
@@ -417,7 +413,7 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
             const int at = rr + 4 * s + q;
             const bool in = at < r1;
             const int m = rows[in ? at : 0];
-            pv[s] = (in && j0 + i < r) ? g.p[(long long)m * r + j] : 0.f;
+            pv[s] = (in && j0 + i < r) ? g.p[(long long)m * g.ldp + j] : 0.f;
             z[s].zero();
             if (in) z[s].load(g, m, c, vec);
         }
@@ -689,7 +685,8 @@ template <> struct Mma<bf16_t> {
     }
     static __device__ __forceinline__ bf16_t part(float v, int lo) {       // high half, and what it leaves
         const bf16_t h = to_bf16(v);
-        return lo ? ((h & 0x7f80u) == 0x7f80u ? (bf16_t)0 : to_bf16(v - up(h))) : h;      // an infinity (or NaN) leaves nothing
+        const float left = (h & 0x7f80u) == 0x7f80u ? 0.f : v - up(h);      // an infinity (or NaN) leaves nothing
+        return to_bf16(lo ? left : v);
     }
 };
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
@@ -740,9 +737,9 @@ struct AdLow {
     const void *in, *v;
     const float* scale;
     const int *order, *key, *seg;
-    float* low;
+    float *low, *t;                         // (M, rp), rp = r rounded up to 4, zeros behind r; t: a copy (M, r) for the caller, or null
     long long ldin, ldv;                    // row pitches; v: (L r) rows
-    int M, C, r, L;
+    int M, C, r, rp, L;
 };
 template <typename T>
 __global__ __launch_bounds__(1024) void k_ad_low(const AdLow a) {
@@ -760,7 +757,11 @@ __global__ __launch_bounds__(1024) void k_ad_low(const AdLow a) {
     const int p = min(first + i, end - 1), m = a.order[p];                         // places past the segment's last row repeat it and write nothing
     if (ad == a.L) {                                                        // no adapter: zero; an id that no adapter has: NaN
         if (live && q == 0)
-            for (int j = wave; j < a.r; j += 16) a.low[(long long)m * a.r + j] = a.key[p] < 0 ? 0.f : nan32();
+            for (int j = wave; j < a.rp; j += 16) {
+                const float v = a.key[p] < 0 ? 0.f : nan32();
+                a.low[(long long)m * a.rp + j] = v;
+                if (a.t && j < a.r) a.t[(long long)m * a.r + j] = v;
+            }
         return;
     }
     const float s = a.scale[ad];
@@ -795,7 +796,10 @@ __global__ __launch_bounds__(1024) void k_ad_low(const AdLow a) {
 #pragma unroll
             for (int w = 0; w < 16; ++w) v += red[w * 256 + tid];
             const int j = j0 + 4 * q + wave;
-            if (live && j < a.r) a.low[(long long)m * a.r + j] = s * v;
+            if (live && j < a.rp) {
+                a.low[(long long)m * a.rp + j] = j < a.r ? s * v : 0.f;
+                if (a.t && j < a.r) a.t[(long long)m * a.r + j] = s * v;
+            }
         }
         __syncthreads();
     }
@@ -808,7 +812,7 @@ template <typename T> struct AdGemm {
     const int *order, *key;
     T* out;
     long long ldin, ldw, vl, vo, vj;        // pitches; strides of v
-    int M, C, O, r, L, tiles_o;             // C: whole chunks
+    int M, C, O, r, rp, L, tiles_o;         // C: whole chunks; rp: low's pitch
     float* partial;                         // with several splits of the reduction (gridDim.y): [split][M][O]
     int per;                                // chunks of a split
 };
@@ -817,7 +821,7 @@ template <typename T> struct AdGemm {
 // with one chunk ahead through registers a chunk of the 128-tile took 2.2 us, the latency of its loads; so 0.46 us (32 KB read from and 16 KB written to LDS
 // for 512 cycles of MFMA).  The 16-byte slot c of row r lies at slot c ^ swizzle(r) (the DMA writes in lane order, so the source address is permuted): a
 // fragment read hits every bank once.  RB = 128 (whole lines, one work-group per CU at BT = 128) where a CU has one tile; RB = 64 (half the LDS: two work-groups
-// per CU, one's start and end under the other's products) where it has more (4,096 rows, 1,024 -> 2,048, bfloat16: 55 -> 44 us).
+// per CU, one's start and end under the other's products) where it has more.
 // After the shared weight's chunks come the adapters': 16-byte piece P of a row belongs to the tile's adapter list[P / pp] and holds E of its ranks (bfloat16: the
 // high halves of all ranks, then the low ones).  The rows of other adapters hold zeros there,
 // and a zero times an infinity or a NaN of a weight would reach them: such weights are staged as zeros and added to their own rows at the end.
@@ -884,56 +888,54 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
             ad_dma16(gx[d] + (long long)c * RB, st + OP + d * 1024);
         }
     };
-    // the adapters' chunks go through registers: raw values first, so that the first of them are loaded under the main loop.  A thread's pieces lie in the same column.
+    // The adapters' chunks go through registers: raw values first, so that the first of them are loaded under the main loop.  A thread's pieces lie in the same column.
+    // Every load is made, from a place that is there, and what does not belong is zeroed at the stash: behind a condition of its own each would be waited for before
+    // the next (4,096 rows, 2,048 -> 1,024, bfloat16, with the conversions and the bias's loads as straight: 37 -> 25 us).
     frag ew[NS];
-    float ex[NS][E];
+    f32x4 ex[NS][E / 4];
     const bool vec_v = a.vj == 1 && a.r % E == 0 && ((uintptr_t)a.v & 15) == 0;
-    int elo = 0;
+    int elo = 0, ead = 0, ej0 = 0;                                          // of the fetched pieces: which half, whose, first rank
+    bool elive = false;
     auto fetch = [&](int c) {
-        const int P = c * PR + tid % PR, ad = P / pp, rem = P - ad * pp, j0 = (rem >= pr ? rem - pr : rem) * E;
+        const int P = c * PR + tid % PR, ad = min(P, ext - 1) / pp, rem = min(P, ext - 1) - ad * pp;
         elo = rem >= pr;
-        const bool live = P < ext;
-        const T* vb = a.v + (live ? (long long)list[ad] : 0ll) * a.vl + j0 * a.vj;
+        ej0 = (elo ? rem - pr : rem) * E;
+        ead = ad;
+        elive = P < ext;
+        const T *vb = a.v + (long long)list[ad] * a.vl, *pv[NS];
+        const float* pl[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            const int row = (tid + 256 * s) / PR, o = o0 + row;
-            const bool mine = live && slot[row] == ad;
-            const float* pl = a.low + (long long)(mine ? rowid[row] : 0) * a.r + j0;
-#pragma unroll
-            for (int k = 0; k < E; ++k) ex[s][k] = 0.f;
-            if (a.r % 4 == 0) {
-#pragma unroll
-                for (int k = 0; k < E; k += 4)
-                    if (mine && j0 + k < a.r) {
-                        const f32x4 u = *(const f32x4*)(pl + k);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) ex[s][k + e] = u[e];
-                    }
-            } else if (mine) {
-#pragma unroll
-                for (int k = 0; k < E; ++k)
-                    if (j0 + k < a.r) ex[s][k] = pl[k];
-            }
-            if (vec_v) {
-#pragma unroll
-                for (int k = 0; k < E; ++k) ew[s][k] = 0;
-                if (live && o < a.O) ew[s] = *(const frag*)(vb + (long long)o * a.vo);
-            } else {
-#pragma unroll
-                for (int k = 0; k < E; ++k) ew[s][k] = (live && o < a.O && j0 + k < a.r) ? vb[(long long)o * a.vo + k * a.vj] : (T)0;
-            }
+            const int row = (tid + 256 * s) / PR;
+            pv[s] = vb + (long long)min(o0 + row, a.O - 1) * a.vo;
+            pl[s] = a.low + (long long)max(rowid[row], 0) * a.rp;
         }
+        if (vec_v) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) ew[s] = *(const frag*)(pv[s] + ej0);
+        } else {
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int k = 0; k < E; ++k) ew[s][k] = pv[s][min(ej0 + k, a.r - 1) * a.vj];
+        }
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int k = 0; k < E; k += 4) ex[s][k / 4] = *(const f32x4*)(pl[s] + min(ej0 + k, a.rp - 4));
     };
     auto stash = [&](int st) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const int e = tid + 256 * s, row = e / PR, at = row * RB + ((e % PR) ^ swizzle(row)) * 16;
-            frag zw = ew[s], zx;
+            const bool mine = elive && slot[row] == ead, out = elive && o0 + row < a.O;
+            frag zw, zx;
             bool ok = true;
 #pragma unroll
             for (int k = 0; k < E; ++k) {
-                ok = ok && finite(zw[k]);
-                zx[k] = X::part(ex[s][k], elo);
+                zw[k] = out && ej0 + k < a.r ? ew[s][k] : (T)0;
+                ok &= finite(zw[k]);
+                zx[k] = X::part(mine && ej0 + k < a.r ? ex[s][k / 4][k & 3] : 0.f, elo);
             }
             if (!ok) {
                 *odd = 1;
@@ -1042,7 +1044,14 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
     const bool vec = a.O % E == 0 && ((uintptr_t)a.out & 15) == 0;
     float bv[E];
 #pragma unroll
-    for (int k = 0; k < E; ++k) bv[k] = (a.bias && !a.partial && o + k < a.O) ? up(a.bias[o + k]) : 0.f;
+    for (int k = 0; k < E; ++k) bv[k] = 0.f;
+    if (a.bias && !a.partial) {                                             // from places that are there: behind conditions each is waited for
+        T bt[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) bt[k] = a.bias[min(o + k, a.O - 1)];
+#pragma unroll
+        for (int k = 0; k < E; ++k) bv[k] = up(bt[k]);
+    }
 #pragma unroll
     for (int v = 0; v < NT; ++v) {
 #pragma unroll
@@ -1070,7 +1079,7 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
                     else if (id >= 0 && o + k < a.O)
                         for (int j = 0; j < a.r; ++j) {
                             const T vv = a.v[id * a.vl + (o + k) * a.vo + j * a.vj];
-                            if (!finite(vv)) z[k] = fmaf(a.low[(long long)m * a.r + j], up(vv), z[k]);
+                            if (!finite(vv)) z[k] = fmaf(a.low[(long long)m * a.rp + j], up(vv), z[k]);
                         }
                 }
             }
@@ -1163,14 +1172,15 @@ static void few_split(int M, int O, int Cn, int* ksplit, int* kw) {
 }
 
 // Tiles of 128 where they fill three quarters of the CUs, else of 64; where those leave CUs idle too, the reduction is split until two work-groups go on each CU, but
-// not under 8 chunks in 32 bits (512 rows, 2,048 -> 1,024, 128 tiles: 44 us unsplit, 28 us and 4 us for the sum in four) and 16 in bfloat16, whose chunk takes an
-// eighth of the matrix time (19 us unsplit, 17.5 + 4 us in four).
+// not under 8 chunks in 32 bits (512 rows, 2,048 -> 1,024, 128 tiles: 42 us unsplit, 27 us and 4 us for the sum in four) and 32 in bfloat16, whose chunk takes an
+// eighth of the matrix time (15 us unsplit, 14 + 4 us in two).  Chunks of 64 bytes (k_ad_gemm's RB) where a CU has several tiles and their rows are short, up to
+// 2,048 bytes (3,000 rows, 1,024 -> 2,048, 1.5 tiles a CU, bfloat16: 26.7 us, 30.2 in chunks of 128; 8,192 rows, 2,048 -> 2,048: 82 and 77 us).
 static void gemm_shape(int M, int O, int Cp, size_t z, int* bt, int* rb, int* splits, int* per) {
     const long long big = (long long)blocks_of(M, 128) * blocks_of(O, 128);
     *bt = big >= 192 ? 128 : 64;
-    *rb = big > 256 && z == 2 ? 64 : 128;
+    *rb = big > 256 && z == 2 && Cp * z <= 2048 ? 64 : 128;
     const int kc = (int)(Cp * z / *rb), tiles = blocks_of(M, *bt) * blocks_of(O, *bt);
-    const int want = tiles >= 256 || *bt == 128 ? 1 : std::max(1, std::min(kc / (z == 4 ? 8 : 16), 512 / tiles));
+    const int want = tiles >= 256 || *bt == 128 ? 1 : std::max(1, std::min(kc / (z == 4 ? 8 : 32), 512 / tiles));
     *per = blocks_of(kc, want);
     *splits = blocks_of(kc, *per);
 }
@@ -1181,11 +1191,12 @@ static size_t gemm_partial(int M, int O, int Cp, size_t z) {
 }
 // the many-row form's rows: whole chunks of 128 bytes, 16-byte aligned
 static inline int padded(int C, size_t z) { const int bk = (int)(128 / z); return (C + bk - 1) / bk * bk; }
+static inline int rank_pitch(int r) { return (r + 3) & ~3; }
 struct FwdWs { size_t t, partial, order, key, seg, xp, wp, ap, total; };
 static FwdWs fwd_ws(int M, int K, int N, int r, int L, size_t z) {
     FwdWs w{};
     size_t o = 0;
-    w.t = o; o += al((size_t)M * r * 4);
+    w.t = o; o += al((size_t)M * rank_pitch(r) * 4);
     if (M <= kFewRows) {
         int ks, kw;
         few_split(M, N, K, &ks, &kw);
@@ -1207,7 +1218,7 @@ struct BwdWs { size_t u, partial, order, key, seg, wt, bt, dyp, part_a, part_b, 
 static BwdWs bwd_ws(int M, int K, int N, int r, int L, size_t z) {
     BwdWs w{};
     size_t o = 0;
-    w.u = o; o += al((size_t)M * r * 4);
+    w.u = o; o += al((size_t)M * rank_pitch(r) * 4);
     if (M <= kFewRows) {
         int ks, kw;
         few_split(M, K, N, &ks, &kw);
@@ -1319,10 +1330,11 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
         lo.v = ws + o.ap; lo.ldv = Kp;
     }
     if (int rc = prepare<T>(pr, st)) return rc;
-    lo.scale = scale; lo.order = pr.order; lo.key = pr.key; lo.seg = pr.seg; lo.low = g.t; lo.M = M; lo.C = Kp; lo.r = r; lo.L = L;
+    lo.scale = scale; lo.order = pr.order; lo.key = pr.key; lo.seg = pr.seg; lo.low = (float*)(ws + o.t); lo.t = t; lo.M = M; lo.C = Kp; lo.r = r;
+    lo.rp = rank_pitch(r); lo.L = L;
     hipLaunchKernelGGL(k_ad_low<T>, dim3(L + 1 + M / 16), dim3(1024), 0, st, lo);
     HMF_LAUNCH_CHECK();
-    m.in = (const T*)lo.in; m.ldin = lo.ldin; m.bias = bias; m.v = b; m.vl = (long long)N * r; m.vo = r; m.vj = 1; m.low = g.t; m.order = pr.order; m.key = pr.key; m.out = y;
+    m.in = (const T*)lo.in; m.ldin = lo.ldin; m.bias = bias; m.v = b; m.vl = (long long)N * r; m.vo = r; m.vj = 1; m.low = lo.low; m.rp = lo.rp; m.order = pr.order; m.key = pr.key; m.out = y;
     m.M = M; m.C = Kp; m.O = N; m.r = r; m.L = L;
     return gemm<T>(m, ws + o.partial, st);
 }
@@ -1335,8 +1347,8 @@ static int backward_t(const T* dy, const void* x, long long ldx, const unsigned 
     g.dy = dy; g.w = w; g.a = a; g.b = b; g.scale = scale; g.ids = ids; g.dx = dx; g.u = (float*)(ws + o.u);
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
     AdGrad ga{}, gb{};
-    ga.p = g.u; ga.z = x; ga.exps = exps; ga.out = da; ga.ldz = ldx; ga.C = ga.Cp = K; ga.trans = 0; ga.blocks = blocks_of(K, 128) * blocks_of(r, 16);
-    gb.p = t; gb.z = dy; gb.out = db; gb.ldz = N; gb.C = gb.Cp = N; gb.trans = 1; gb.blocks = blocks_of(N, 128) * blocks_of(r, 16);
+    ga.p = g.u; ga.ldp = r; ga.z = x; ga.exps = exps; ga.out = da; ga.ldz = ldx; ga.C = ga.Cp = K; ga.trans = 0; ga.blocks = blocks_of(K, 128) * blocks_of(r, 16);
+    gb.p = t; gb.ldp = r; gb.z = dy; gb.out = db; gb.ldz = N; gb.C = gb.Cp = N; gb.trans = 1; gb.blocks = blocks_of(N, 128) * blocks_of(r, 16);
     const int V = 16 / (int)sizeof(T);
     const bool vec = N % V == 0 && !off16(dy);
     if (M <= kFewRows) {
@@ -1368,12 +1380,14 @@ static int backward_t(const T* dy, const void* x, long long ldx, const unsigned 
     }
     if (int rc = prepare<T>(pr, st)) return rc;
     AdLow lo{};
-    lo.in = dyp; lo.ldin = Np; lo.v = ws + o.bt; lo.ldv = Np; lo.scale = scale; lo.order = pr.order; lo.key = pr.key; lo.seg = pr.seg; lo.low = g.u; lo.M = M; lo.C = Np; lo.r = r; lo.L = L;
+    lo.in = dyp; lo.ldin = Np; lo.v = ws + o.bt; lo.ldv = Np; lo.scale = scale; lo.order = pr.order; lo.key = pr.key; lo.seg = pr.seg; lo.low = g.u; lo.M = M; lo.C = Np; lo.r = r;
+    lo.rp = rank_pitch(r); lo.L = L;
+    ga.ldp = lo.rp;
     hipLaunchKernelGGL(k_ad_low<T>, dim3(L + 1 + M / 16), dim3(1024), 0, st, lo);
     HMF_LAUNCH_CHECK();
     if (dx) {
         AdGemm<T> m{};
-        m.in = dyp; m.ldin = Np; m.w = (const T*)(ws + o.wt); m.ldw = Np; m.v = a; m.vl = (long long)r * K; m.vo = 1; m.vj = K; m.low = g.u; m.order = pr.order; m.key = pr.key;
+        m.in = dyp; m.ldin = Np; m.w = (const T*)(ws + o.wt); m.ldw = Np; m.v = a; m.vl = (long long)r * K; m.vo = 1; m.vj = K; m.low = g.u; m.rp = lo.rp; m.order = pr.order; m.key = pr.key;
         m.out = dx; m.M = M; m.C = Np; m.O = K; m.r = r; m.L = L;
         if (int rc = gemm<T>(m, ws + o.partial, st)) return rc;
     }
