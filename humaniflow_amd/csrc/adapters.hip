@@ -32,6 +32,11 @@ constexpr int kMaxRank = 64;
 __device__ __forceinline__ float up(float v) { return v; }
 __device__ __forceinline__ float up(bf16_t h) { return __uint_as_float((unsigned)h << 16); }
 __device__ __forceinline__ bf16_t to_bf16(float f) { return __builtin_bit_cast(bf16_t, (__bf16)f); }      // nearest even, one instruction (a NaN stays one)
+// a number less its nearest bfloat16 (exact; an infinity or NaN leaves nothing): 8 of its 24 bits at a time
+__device__ __forceinline__ float bf16_left(float v) {
+    const bf16_t h = to_bf16(v);
+    return (h & 0x7f80u) == 0x7f80u ? 0.f : v - up(h);
+}
 __device__ __forceinline__ void down(float* p, float v) { *p = v; }
 __device__ __forceinline__ void down(bf16_t* p, float v) { *p = to_bf16(v); }
 
@@ -308,7 +313,9 @@ __global__ __launch_bounds__(64) void k_ad_join(const AdArgs<T> a) {
 // ---------------------------------------------------------------------------------------------------
 // gradients of the adapters: G[j][c] = sum over an adapter's rows of p[m][j] z[m][c], p (M, r) in 32 bits;  dA: p = u, z = x (or its 8-bit checkpoint);  dB^T: p = t, z = dy.
 // A work-group owns (adapter, piece of <= 256 of its rows, 128 columns, 16 ranks); its waves take a part of the rows each, 4 rows per 16 x 16 x 4 MFMA step, and every lane the
-// eight columns 8 i .. 8 i + 7 (one load of 8 to 32 bytes feeds eight MFMA tiles); they meet in LDS in a fixed order.  More pieces than one: partial sums in the
+// eight columns 8 i .. 8 i + 7 (one load of 8 to 32 bytes feeds eight MFMA tiles); they meet in LDS in a fixed order.  In bfloat16 z is exact in 16 bits (a
+// checkpoint's value too), so p goes in as three parts of 8 bits
+// and 32 rows take three 16 x 16 x 32 steps, a fifth of the matrix time.  More pieces than one: partial sums in the
 // workspace, joined by k_ad_grad_join.  Tiles of 32 ranks (32 x 32 x 2) waste half the matrix work at the usual ranks of up to 16.
 // ---------------------------------------------------------------------------------------------------
 struct AdGrad {
@@ -321,106 +328,136 @@ struct AdGrad {
     int C, Cp, trans, blocks;          // columns, columns that may be read; blocks: blocks of 128 columns x 16 ranks, columns first
 };
 
-// eight consecutive elements of a row of z, as they lie in memory; columns past C read as zero
+// Eight consecutive elements of a row of z, as they lie in memory; past the last column there is no promise but that the memory is there (nothing of it is stored).
 template <typename T, bool ACT8> struct Z8;
-template <> struct Z8<float, false> {
-    f32x4 d[2];
-    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.ldz % 4 == 0 && g.Cp % 8 == 0 && ((uintptr_t)g.z & 15) == 0; }
-    __device__ __forceinline__ void load(const AdGrad& g, int m, int c, bool vec) {
-        const float* p = (const float*)g.z + (long long)m * g.ldz + c;
-        if (vec) {
-            if (c < g.C) { d[0] = *(const f32x4*)p; d[1] = *(const f32x4*)(p + 4); }
-        } else {
+template <typename T> struct Z8<T, false> {
+    typedef __attribute__((ext_vector_type(8))) T v8;
+    v8 d;
+    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.ldz % (16 / sizeof(T)) == 0 && g.Cp % 8 == 0 && ((uintptr_t)g.z & 15) == 0; }
+    __device__ __forceinline__ void load(const AdGrad& g, int m, int c) {
+        const uint4* p = (const uint4*)((const T*)g.z + (long long)m * g.ldz + min(c, g.Cp - 8));
+        uint4 h[sizeof(T) / 2];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (c + k < g.C) d[k >> 2][k & 3] = p[k];
-        }
+        for (int k = 0; k < (int)sizeof(T) / 2; ++k) h[k] = p[k];
+        __builtin_memcpy(&d, h, sizeof(d));
     }
-    __device__ __forceinline__ void zero() { d[0] = d[1] = f32x4{0.f, 0.f, 0.f, 0.f}; }
-    __device__ __forceinline__ float get(int k) const { return d[k >> 2][k & 3]; }
-};
-template <> struct Z8<bf16_t, false> {
-    u16x8 d;
-    static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.ldz % 8 == 0 && g.Cp % 8 == 0 && ((uintptr_t)g.z & 15) == 0; }
-    __device__ __forceinline__ void load(const AdGrad& g, int m, int c, bool vec) {
-        const bf16_t* p = (const bf16_t*)g.z + (long long)m * g.ldz + c;
-        if (vec) {
-            if (c < g.C) d = *(const u16x8*)p;
-        } else {
+    __device__ __forceinline__ void load_any(const AdGrad& g, int m, int c) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (c + k < g.C) d[k] = p[k];
-        }
+        for (int k = 0; k < 8; ++k) d[k] = ((const T*)g.z)[(long long)m * g.ldz + min(c + k, g.C - 1)];
     }
-    __device__ __forceinline__ void zero() {
+    __device__ __forceinline__ void keep(bool in) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) d[k] = 0;
+        for (int k = 0; k < 8; ++k) d[k] = in ? d[k] : (T)0;
     }
-    __device__ __forceinline__ float get(int k) const { return up(d[k]); }
+    __device__ __forceinline__ float get(int k) const { return up((T)d[k]); }
+    __device__ __forceinline__ bf16_t half(int k) const { return d[k]; }   // bfloat16 alone
+    static __device__ __forceinline__ float one(const AdGrad& g, int m, int c) { return up(((const T*)g.z)[(long long)m * g.ldz + c]); }
 };
 template <typename T> struct Z8<T, true> {
     unsigned int w[2], e[2];
     static __device__ __forceinline__ bool aligned(const AdGrad& g) { return g.C % 8 == 0 && ((uintptr_t)g.z & 7) == 0 && ((uintptr_t)g.exps & 7) == 0; }
-    __device__ __forceinline__ void load(const AdGrad& g, int m, int c, bool vec) {
-        const unsigned char* pc = (const unsigned char*)g.z + (long long)m * g.C + c;
-        const unsigned char* pe = g.exps + (long long)(m >> 5) * g.C + c;
-        if (vec) {
-            if (c < g.C) {
-                const uint2 a = *(const uint2*)pc, b = *(const uint2*)pe;
-                w[0] = a.x; w[1] = a.y; e[0] = b.x; e[1] = b.y;
-            }
-        } else {
+    __device__ __forceinline__ void load(const AdGrad& g, int m, int c) {
+        const int at = min(c, g.C - 8);
+        const uint2 a = *(const uint2*)((const unsigned char*)g.z + (long long)m * g.C + at), b = *(const uint2*)(g.exps + (long long)(m >> 5) * g.C + at);
+        w[0] = a.x; w[1] = a.y; e[0] = b.x; e[1] = b.y;
+    }
+    __device__ __forceinline__ void load_any(const AdGrad& g, int m, int c) {
+        w[0] = w[1] = e[0] = e[1] = 0u;
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (c + k < g.C) { w[k >> 2] |= (unsigned)pc[k] << (8 * (k & 3)); e[k >> 2] |= (unsigned)pe[k] << (8 * (k & 3)); }
+        for (int k = 0; k < 8; ++k) {
+            const int at = min(c + k, g.C - 1);
+            w[k >> 2] |= (unsigned)((const unsigned char*)g.z)[(long long)m * g.C + at] << (8 * (k & 3));
+            e[k >> 2] |= (unsigned)g.exps[(long long)(m >> 5) * g.C + at] << (8 * (k & 3));
         }
     }
-    __device__ __forceinline__ void zero() { w[0] = w[1] = e[0] = e[1] = 0u; }
+    __device__ __forceinline__ void keep(bool in) {
+        w[0] = in ? w[0] : 0u;
+        w[1] = in ? w[1] : 0u;
+    }
     __device__ __forceinline__ float get(int k) const {
         const int q = (int)(signed char)(w[k >> 2] >> (8 * (k & 3)));
         const float step = __uint_as_float((unsigned)max((int)((e[k >> 2] >> (8 * (k & 3))) & 0xffu) - 6, 0) << 23);
         return q == -128 ? nan32() : (float)q * step;
     }
+    __device__ __forceinline__ bf16_t half(int k) const { return (bf16_t)(__float_as_uint(get(k)) >> 16); }      // exact: seven bits times a power of two
+    static __device__ __forceinline__ float one(const AdGrad& g, int m, int c) {
+        Z8<T, true> z;
+        z.w[0] = ((const unsigned char*)g.z)[(long long)m * g.C + c];
+        z.e[0] = g.exps[(long long)(m >> 5) * g.C + c];
+        return z.get(0);
+    }
 };
 
-constexpr int grad_lds(int waves) { return waves * 32 * 64; }          // floats
-// T: type of z and of the gradients; ACT8: z is a checkpoint; NW: waves of the work-group (4 or 8)
-template <typename T, bool ACT8, int NW>
+constexpr int kGradLds = 4 * 32 * 64;                                     // floats
+// T: type of z and of the gradients; ACT8: z is a checkpoint.  Four waves (4,096 rows, 2,048 -> 1,024, 16 adapters, bfloat16: 12.7 us; eight, of which a CU holds
+// one work-group: 14.7, and 16.6 with z and p in 32 bits)
+template <typename T, bool ACT8>
 __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* rows, int n, int l, long long piece, bool whole, int block, float* red) {
     const int ncb = (g.C + 127) / 128, cb = block % ncb, j0 = block / ncb * 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const int c = cb * 128 + 8 * i;
     if (n == 0) {                                                          // an adapter without rows has one piece: its part of the result is zero
         const int c0 = cb * 128, w = min(128, g.C - c0), nj = min(16, r - j0);
-        for (int e = threadIdx.x; e < 128 * 16; e += NW * 64) {
+        for (int e = threadIdx.x; e < 128 * 16; e += 256) {
             const int jj = g.trans ? e & 15 : e >> 7, cc = g.trans ? e >> 4 : e & 127;      // along what lies next to each other
             if (jj < nj && cc < w) down((T*)g.out + (g.trans ? ((long long)l * g.C + c0 + cc) * r + j0 + jj : ((long long)l * r + j0 + jj) * g.C + c0 + cc), 0.f);
         }
         return;
     }
     const bool vec = Z8<T, ACT8>::aligned(g);
-    const int per = ((n + NW - 1) / NW + 3) & ~3, r0 = wave * per, r1 = min(r0 + per, n);
+    const int per = ((n + 3) / 4 + 3) & ~3, r0 = wave * per, r1 = min(r0 + per, n);
     const int j = min(j0 + i, r - 1);
     f32x4 acc[8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     constexpr int U = 8;
+    constexpr bool B16 = sizeof(T) == 2;
+    auto place = [&](int s) { return B16 ? 8 * q + s : 4 * s + q; };       // of a lane's row s among the 32; bfloat16: the eight that its operand holds
     for (int rr = r0; rr < r1; rr += 4 * U) {
         Z8<T, ACT8> z[U];
         float pv[U];
+        int m[U];
 #pragma unroll
-        for (int s = 0; s < U; ++s) {
-            const int at = rr + 4 * s + q;
-            const bool in = at < r1;
-            const int m = rows[in ? at : 0];
-            pv[s] = (in && j0 + i < r) ? g.p[(long long)m * g.ldp + j] : 0.f;
-            z[s].zero();
-            if (in) z[s].load(g, m, c, vec);
+        for (int s = 0; s < U; ++s) m[s] = rows[min(rr + place(s), r1 - 1)];
+        if (vec) {                                                         // every load is made, behind conditions each would be waited for before the next
+#pragma unroll
+            for (int s = 0; s < U; ++s) z[s].load(g, m[s], c);
+        } else {
+#pragma unroll
+            for (int s = 0; s < U; ++s) z[s].load_any(g, m[s], c);
         }
 #pragma unroll
-        for (int s = 0; s < U; ++s)
+        for (int s = 0; s < U; ++s) pv[s] = g.p[(long long)m[s] * g.ldp + j];
 #pragma unroll
-            for (int t = 0; t < 8; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[s], z[s].get(t), acc[t], 0, 0, 0);
+        for (int s = 0; s < U; ++s) {
+            const bool in = rr + place(s) < r1;
+            z[s].keep(in);                                                 // not an infinity of the last row times zero
+            pv[s] = in && j0 + i < r ? pv[s] : 0.f;
+        }
+        if constexpr (B16) {
+            u16x8 part[3];                                                 // smallest first
+#pragma unroll
+            for (int k = 2; k >= 0; --k)
+#pragma unroll
+                for (int s = 0; s < U; ++s) {
+                    part[k][s] = to_bf16(pv[s]);
+                    pv[s] = bf16_left(pv[s]);
+                }
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                u16x8 v;
+#pragma unroll
+                for (int s = 0; s < U; ++s) v[s] = z[s].half(t);
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, part[k]), __builtin_bit_cast(bf16x8, v), acc[t], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < U; ++s)
+#pragma unroll
+                for (int t = 0; t < 8; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[s], z[s].get(t), acc[t], 0, 0, 0);
+        }
     }
     // element e of tile t: rank j0 + 4 q + e of column c + t
 #pragma unroll
@@ -432,13 +469,21 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
         const int at = (t * 4 + e) * 64 + lane;
         float v = red[at];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) v += red[at + w * 32 * 64];
+        for (int w = 1; w < 4; ++w) v += red[at + w * 32 * 64];
+        if constexpr (B16) {                                           // an infinity of z times the parts of p may be a NaN that their sum's product is not
+            const int jj = j0 + 4 * q + e, cc = c + t;
+            if (v != v && jj < r && cc < g.C) {
+                v = 0.f;
+#pragma unroll 4
+                for (int k = 0; k < n; ++k) v = fmaf(g.p[(long long)rows[k] * g.ldp + jj], Z8<T, ACT8>::one(g, rows[k], cc), v);
+            }
+        }
         return v;
     };
-    if (whole && g.trans) {                                            // a wave: 8 / NW columns, four ranks each
+    if (whole && g.trans) {                                            // a wave: two columns, four ranks each
 #pragma unroll
-        for (int t2 = 0; t2 < 8 / NW; ++t2) {
-            const int t = 8 / NW * wave + t2, jj = j0 + 4 * q;
+        for (int t2 = 0; t2 < 2; ++t2) {
+            const int t = 2 * wave + t2, jj = j0 + 4 * q;
             T* po = (T*)g.out + ((long long)l * g.C + c + t) * r + jj;
             T h[4] __attribute__((aligned(16)));
 #pragma unroll
@@ -456,34 +501,31 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
                 }
             }
         }
-    } else {                                                           // a wave: rank j0 + 4 q + (w & 3), TN columns
-        constexpr int TN = 32 / NW;
-        const int e = wave & 3, t0 = (wave >> 2) * TN, jj = j0 + 4 * q + e, c0 = c + t0;
-        float v[TN];
+    } else {                                                           // a wave: rank j0 + 4 q + wave, eight columns
+        const int e = wave, jj = j0 + 4 * q + e;
+        float v[8];
 #pragma unroll
-        for (int t = 0; t < TN; ++t) v[t] = total(t0 + t, e);
+        for (int t = 0; t < 8; ++t) v[t] = total(t, e);
         if (jj < r) {
             if (!whole) {
-                float* po = g.part + (piece * r + jj) * g.C + c0;
+                float* po = g.part + (piece * r + jj) * g.C + c;
 #pragma unroll
-                for (int t = 0; t < TN; ++t)
-                    if (c0 + t < g.C) po[t] = v[t];
+                for (int t = 0; t < 8; ++t)
+                    if (c + t < g.C) po[t] = v[t];
             } else {
-                T* po = (T*)g.out + ((long long)l * r + jj) * g.C + c0;
-                T h[TN] __attribute__((aligned(16)));
+                T* po = (T*)g.out + ((long long)l * r + jj) * g.C + c;
+                T h[8] __attribute__((aligned(16)));
 #pragma unroll
-                for (int t = 0; t < TN; ++t) down(h + t, v[t]);
+                for (int t = 0; t < 8; ++t) down(h + t, v[t]);
                 if (g.C % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {
-                    if (c0 < g.C) {
-                        if (sizeof(h) == 8) *(uint2*)po = *(const uint2*)h;
-                        else
+                    if (c < g.C) {
 #pragma unroll
-                            for (int k = 0; k < (int)sizeof(h) / 16; ++k) *((uint4*)po + k) = *((const uint4*)h + k);
+                        for (int k = 0; k < (int)sizeof(h) / 16; ++k) *((uint4*)po + k) = *((const uint4*)h + k);
                     }
                 } else {
 #pragma unroll
-                    for (int t = 0; t < TN; ++t)
-                        if (c0 + t < g.C) po[t] = h[t];
+                    for (int t = 0; t < 8; ++t)
+                        if (c + t < g.C) po[t] = h[t];
                 }
             }
         }
@@ -508,7 +550,7 @@ __device__ __forceinline__ int rows_of(const int* ids, int M, int l, int* rows, 
 // few rows, backward, first launch: dx's partial sums, u, dB
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_ad_few_back(const AdArgs<T> a, const AdGrad db, int tiles_o, int tiles_m) {
-    __shared__ float red[grad_lds(4)];
+    __shared__ float red[kGradLds];
     __shared__ int rows[kFewRows], cnt[4];
     const int nb = a.dx ? tiles_o * a.ksplit * tiles_m : 0;
     int id = blockIdx.x;
@@ -525,13 +567,13 @@ __global__ __launch_bounds__(256) void k_ad_few_back(const AdArgs<T> a, const Ad
     id -= a.M;
     const int l = id / db.blocks;
     const int n = rows_of(a.ids, a.M, l, rows, cnt);
-    grad_piece<T, false, 4>(db, a.r, rows, n, l, 0, true, id - l * db.blocks, red);
+    grad_piece<T, false>(db, a.r, rows, n, l, 0, true, id - l * db.blocks, red);
 }
 
 // second launch: dx = partial sums + A_l^T u, dA
 template <typename T, bool ACT8>
 __global__ __launch_bounds__(256) void k_ad_few_back2(const AdArgs<T> a, const AdGrad da, int join_wgs) {
-    __shared__ float red[grad_lds(4)];
+    __shared__ float red[kGradLds];
     __shared__ int rows[kFewRows], cnt[4];
     int id = blockIdx.x;
     if (id < join_wgs) {
@@ -548,7 +590,7 @@ __global__ __launch_bounds__(256) void k_ad_few_back2(const AdArgs<T> a, const A
     id -= join_wgs;
     const int l = id / da.blocks;
     const int n = rows_of(a.ids, a.M, l, rows, cnt);
-    grad_piece<T, ACT8, 4>(da, a.r, rows, n, l, 0, true, id - l * da.blocks, red);
+    grad_piece<T, ACT8>(da, a.r, rows, n, l, 0, true, id - l * da.blocks, red);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -683,11 +725,7 @@ template <> struct Mma<bf16_t> {
     static __device__ __forceinline__ f32x4 mma16(frag a, frag b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ bf16_t part(float v, int lo) {       // high half, and what it leaves
-        const bf16_t h = to_bf16(v);
-        const float left = (h & 0x7f80u) == 0x7f80u ? 0.f : v - up(h);      // an infinity (or NaN) leaves nothing
-        return to_bf16(lo ? left : v);
-    }
+    static __device__ __forceinline__ bf16_t part(float v, int lo) { return to_bf16(lo ? bf16_left(v) : v); }      // high half, and what it leaves
 };
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ bool finite(bf16_t v) { return (v & 0x7f80u) != 0x7f80u; }
@@ -1116,8 +1154,8 @@ __global__ __launch_bounds__(256) void k_ad_sum(const float* __restrict__ partia
 }
 
 template <typename T, bool ACT8>
-__global__ __launch_bounds__(512) void k_ad_grads(const AdGrad da, const AdGrad db, const int* __restrict__ order, const int* __restrict__ seg, int r, int L) {
-    __shared__ float red[grad_lds(8)];
+__global__ __launch_bounds__(256) void k_ad_grads(const AdGrad da, const AdGrad db, const int* __restrict__ order, const int* __restrict__ seg, int r, int L) {
+    __shared__ float red[kGradLds];
     __shared__ int rows[kFewRows];
     int l, np, s0, end;
     find_piece<kFewRows, 1>(seg, L, blockIdx.y, l, np, s0, end);
@@ -1126,8 +1164,8 @@ __global__ __launch_bounds__(512) void k_ad_grads(const AdGrad da, const AdGrad 
     if ((int)threadIdx.x < n) rows[threadIdx.x] = order[s0 + threadIdx.x];
     __syncthreads();
     const int cb = blockIdx.x;
-    if (cb < da.blocks) grad_piece<T, ACT8, 8>(da, r, rows, n, l, blockIdx.y, np == 1, cb, red);
-    else grad_piece<T, false, 8>(db, r, rows, n, l, blockIdx.y, np == 1, cb - da.blocks, red);
+    if (cb < da.blocks) grad_piece<T, ACT8>(da, r, rows, n, l, blockIdx.y, np == 1, cb, red);
+    else grad_piece<T, false>(db, r, rows, n, l, blockIdx.y, np == 1, cb - da.blocks, red);
 }
 
 // sums of the adapters that had several pieces, in the pieces' order; a column of work-groups per adapter, gone at once where there is nothing to add
@@ -1395,8 +1433,8 @@ static int backward_t(const T* dy, const void* x, long long ldx, const unsigned 
     ga.part = (float*)(ws + o.part_a);
     gb.part = (float*)(ws + o.part_b);
     const dim3 grid(ga.blocks + gb.blocks, L + M / kFewRows);
-    if (exps) hipLaunchKernelGGL((k_ad_grads<T, true>), grid, dim3(512), 0, st, ga, gb, order, seg, r, L);
-    else hipLaunchKernelGGL((k_ad_grads<T, false>), grid, dim3(512), 0, st, ga, gb, order, seg, r, L);
+    if (exps) hipLaunchKernelGGL((k_ad_grads<T, true>), grid, dim3(256), 0, st, ga, gb, order, seg, r, L);
+    else hipLaunchKernelGGL((k_ad_grads<T, false>), grid, dim3(256), 0, st, ga, gb, order, seg, r, L);
     HMF_LAUNCH_CHECK();
     hipLaunchKernelGGL(k_ad_grad_join<T>, dim3(std::min(256, blocks_of((long long)r * (K + N), 256)), L), dim3(256), 0, st, ga, gb, seg, r, L);
     HMF_LAUNCH_CHECK();

@@ -148,6 +148,24 @@ def test_infinite_weight_of_one_rank_is_added_to_its_rows():
         assert torch.equal(y[rows][:, 5].float(), want) and torch.isfinite(y[~rows]).all()
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('M', [6, 300])
+def test_infinite_gradient_of_one_output(M, dtype):
+    """An infinity in dy is one in the gradients that it reaches (times t, u and x that are not zero), in both forms, and reaches no other adapter."""
+    c = _case(M, 64, 48, 4, 2, 'one', dtype, 1)
+    c['ids'] = (torch.arange(M) % 2).to(torch.int32).cuda()
+    t = adapters.adapted_linear_forward(**c)[1]
+    dy = torch.randn(M, 48, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    args = (c['weight'], c['A'], c['B'], c['scale'], c['ids'])
+    _, cA, cB = adapters.adapted_linear_backward(dy, c['x'], t, *args)
+    dy[1, 5] = float('inf')
+    _, dA, dB = adapters.adapted_linear_backward(dy, c['x'], t, *args)
+    assert torch.equal(dA[0], cA[0]) and torch.equal(dB[0], cB[0])
+    inf = torch.full((), float('inf'), device='cuda', dtype=dtype)
+    assert torch.equal(dB[1, 5], torch.copysign(inf, t[1].to(dtype))) and torch.equal(dB[1, 6:], cB[1, 6:]) and torch.equal(dB[1, :5], cB[1, :5])
+    assert torch.equal(dA[1], torch.copysign(inf, c['B'][1, 5][:, None] * c['x'][1][None, :]))
+
+
 def test_empty_and_refused():
     c = _case(4, 64, 48, 4, 2, 'mixed', torch.float32, 0)
     y = adapters.adapted_linear(**{**c, 'x': c['x'][:0], 'ids': c['ids'][:0]})
