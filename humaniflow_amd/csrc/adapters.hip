@@ -40,31 +40,19 @@ __device__ __forceinline__ float bf16_left(float v) {
 __device__ __forceinline__ void down(float* p, float v) { *p = v; }
 __device__ __forceinline__ void down(bf16_t* p, float v) { *p = to_bf16(v); }
 
-// four consecutive elements at p as floats, `n` of them valid (VEC: the caller guarantees alignment, and n is 0 or >= 4)
-template <bool VEC> __device__ __forceinline__ f32x4 load4(const float* p, int n) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (VEC) {
-        if (n > 0) v = *(const f32x4*)p;
-    } else {
+// Four consecutive elements at p as floats, `n` of them valid and zero behind; n <= 0: none.  Every load is made, at the last valid place where its own is none (at least one
+// element, VEC: four, lies in front of p + n): behind conditions each would be waited for before the next (4 rows, 1,940 -> 1,379, rank 15, bfloat16: 78 us).
+// VEC: the caller guarantees alignment, and n is a multiple of 4.
+template <bool VEC, typename T> __device__ __forceinline__ f32x4 load4(const T* p, int n) {
+    typedef __attribute__((ext_vector_type(4))) T t4;
+    t4 h;
+    if (VEC) h = *(const t4*)(p + (n > 0 ? 0 : n - 4));
+    else
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < n) v[k] = p[k];
-    }
-    return v;
-}
-template <bool VEC> __device__ __forceinline__ f32x4 load4(const bf16_t* p, int n) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (VEC) {
-        if (n > 0) {
-            const u16x4 h = *(const u16x4*)p;
+        for (int k = 0; k < 4; ++k) h[k] = p[min(k, n - 1)];
+    f32x4 v;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = up(h[k]);
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < n) v[k] = up(p[k]);
-    }
+    for (int k = 0; k < 4; ++k) v[k] = k < n ? up((T)h[k]) : 0.f;
     return v;
 }
 __device__ __forceinline__ float wave_sum(float v) {
@@ -101,14 +89,20 @@ __device__ __forceinline__ void low_row(const AdArgs<T>& a, int m, float* t) {
     const float s = a.scale[l];
     for (int j0 = wave * 4; j0 < a.r; j0 += 16) {
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int k = lane * 4; k < a.K; k += 256) {
-            const f32x4 xv = load4<VEC>(xr + k, a.K - k);
+        for (int k0 = lane * 4; k0 - lane * 4 < a.K; k0 += 512) {          // ten loads in flight
+            f32x4 xv[2], av[2][4];
 #pragma unroll
-            for (int jj = 0; jj < 4; ++jj) {
-                const int j = min(j0 + jj, a.r - 1);
-                const f32x4 av = load4<VEC>(al + (long long)j * a.K + k, a.K - k);
-                acc[jj] = fmaf(xv[0], av[0], fmaf(xv[1], av[1], fmaf(xv[2], av[2], fmaf(xv[3], av[3], acc[jj]))));
+            for (int h = 0; h < 2; ++h) {
+                const int k = k0 + 256 * h;
+                xv[h] = load4<VEC>(xr + k, a.K - k);
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) av[h][jj] = load4<VEC>(al + (long long)min(j0 + jj, a.r - 1) * a.K + k, a.K - k);
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj)
+                    acc[jj] = fmaf(xv[h][0], av[h][jj][0], fmaf(xv[h][1], av[h][jj][1], fmaf(xv[h][2], av[h][jj][2], fmaf(xv[h][3], av[h][jj][3], acc[jj]))));
         }
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
@@ -178,7 +172,10 @@ __device__ __forceinline__ void base_tile(const AdArgs<T>& a, const T* in, long 
                 wv[g] = load4<VEC>(a.w + (long long)oc * Cn + cc, n);
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) wv[g][e] = e < n ? up(a.w[(long long)(cc + e) * O + oc]) : 0.f;
+                for (int e = 0; e < 4; ++e) {
+                    const T h = a.w[(long long)min(cc + e, c1 - 1) * O + oc];
+                    wv[g][e] = e < n ? up(h) : 0.f;
+                }
             }
         }
 #pragma unroll
@@ -214,8 +211,9 @@ __global__ __launch_bounds__(256) void k_ad_few(const AdArgs<T> a, int tiles_o, 
 }
 
 // One to four rows (a single image): everything in ONE launch, since a second one costs as much as the work.  A work-group finds the rows' t itself -- A_l is read once per
-// work-group, from L2 -- and then its waves two outputs each, lanes along K.  1 row, 2,048 -> 1,024, rank 16 in 32 bits: 9 us and two launches in the form below.
-constexpr int kOneRows = 4, kOneBytes = 512 << 10;                          // rows; bytes of A that a work-group reads for them
+// work-group, from L2 -- and then its waves two outputs each, lanes along K.  1 row, 2,048 -> 1,024, rank 16 in 32 bits: 7.6 us, and two launches of 9 us in all in the form below.
+constexpr int kOneRows = 4, kOneBytes = 512 << 10, kOneOdd = 64 << 10;      // rows; bytes of A that a work-group reads for them, and where its rows are not aligned (4 rows, 1,941 ->
+// 1,379, rank 15: 56 us, 18 below; 4 rows, 1,001 -> 64, rank 8, bfloat16: 16 us, 18 below)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_ad_one(const AdArgs<T> a) {
     __shared__ float st[kOneRows][kMaxRank];
@@ -226,18 +224,28 @@ __global__ __launch_bounds__(256) void k_ad_one(const AdArgs<T> a) {
 #pragma unroll
     for (int m = 0; m < kOneRows; ++m) y[m][0] = y[m][1] = 0.f;
     const T *w0 = a.w + (long long)min(n0, a.N - 1) * a.K, *w1 = a.w + (long long)min(n0 + 1, a.N - 1) * a.K;
-    for (int k = lane * 4; k < a.K; k += 256) {
-        const f32x4 u0 = load4<VEC>(w0 + k, a.K - k), u1 = load4<VEC>(w1 + k, a.K - k);
+    for (int k0 = lane * 4; k0 - lane * 4 < a.K; k0 += 1024) {             // the weight's loads of four steps in flight
+        f32x4 u0[4], u1[4];
 #pragma unroll
-        for (int m = 0; m < kOneRows; ++m)
-            if (m < a.M) {
-                const f32x4 xv = load4<VEC>(a.x + m * a.ldx + k, a.K - k);
+        for (int h = 0; h < 4; ++h) {
+            const int k = k0 + 256 * h;
+            u0[h] = load4<VEC>(w0 + k, a.K - k);
+            u1[h] = load4<VEC>(w1 + k, a.K - k);
+        }
+#pragma unroll
+        for (int m = 0; m < kOneRows; ++m) {
+            if (m >= a.M) break;
+            f32x4 xv[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) xv[h] = load4<VEC>(a.x + m * a.ldx + k0 + 256 * h, a.K - k0 - 256 * h);
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    y[m][0] = fmaf(xv[e], u0[e], y[m][0]);
-                    y[m][1] = fmaf(xv[e], u1[e], y[m][1]);
+                    y[m][0] = fmaf(xv[h][e], u0[h][e], y[m][0]);
+                    y[m][1] = fmaf(xv[h][e], u1[h][e], y[m][1]);
                 }
-            }
+        }
     }
     for (int m = 0; m < a.M; ++m) {
         low_row<T, VEC>(a, m, st[m]);
@@ -312,8 +320,8 @@ __global__ __launch_bounds__(64) void k_ad_join(const AdArgs<T> a) {
 
 // ---------------------------------------------------------------------------------------------------
 // gradients of the adapters: G[j][c] = sum over an adapter's rows of p[m][j] z[m][c], p (M, r) in 32 bits;  dA: p = u, z = x (or its 8-bit checkpoint);  dB^T: p = t, z = dy.
-// A work-group owns (adapter, piece of <= 256 of its rows, 128 columns, 16 ranks); its waves take a part of the rows each, 4 rows per 16 x 16 x 4 MFMA step, and every lane the
-// eight columns 8 i .. 8 i + 7 (one load of 8 to 32 bytes feeds eight MFMA tiles); they meet in LDS in a fixed order.  In bfloat16 z is exact in 16 bits (a
+// A work-group owns (adapter, piece of <= 256 of its rows, 128 columns, 16 ranks); its waves take a part of the rows each, 4 rows per 16 x 16 x 4 MFMA step, and every lane
+// eight columns, 8 i .. 8 i + 7 where z is aligned (one load of 8 to 32 bytes feeds eight MFMA tiles); they meet in LDS in a fixed order.  In bfloat16 z is exact in 16 bits (a
 // checkpoint's value too), so p goes in as three parts of 8 bits
 // and 32 rows take three 16 x 16 x 32 steps, a fifth of the matrix time.  More pieces than one: partial sums in the
 // workspace, joined by k_ad_grad_join.  Tiles of 32 ranks (32 x 32 x 2) waste half the matrix work at the usual ranks of up to 16.
@@ -328,7 +336,8 @@ struct AdGrad {
     int C, Cp, trans, blocks;          // columns, columns that may be read; blocks: blocks of 128 columns x 16 ranks, columns first
 };
 
-// Eight consecutive elements of a row of z, as they lie in memory; past the last column there is no promise but that the memory is there (nothing of it is stored).
+// Eight elements of a row of z, as they lie in memory: consecutive ones (`load`), or, where the rows are not aligned, every sixteenth (`load_any`, in order over the
+// lanes; a row of 1,230 in 32 bits, 462 rows, 40 adapters, consecutive: 47 us).  Past the last column there is no promise but that the memory is there (nothing of it is stored).
 template <typename T, bool ACT8> struct Z8;
 template <typename T> struct Z8<T, false> {
     typedef __attribute__((ext_vector_type(8))) T v8;
@@ -343,7 +352,7 @@ template <typename T> struct Z8<T, false> {
     }
     __device__ __forceinline__ void load_any(const AdGrad& g, int m, int c) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) d[k] = ((const T*)g.z)[(long long)m * g.ldz + min(c + k, g.C - 1)];
+        for (int k = 0; k < 8; ++k) d[k] = ((const T*)g.z)[(long long)m * g.ldz + min(c + 16 * k, g.C - 1)];
     }
     __device__ __forceinline__ void keep(bool in) {
 #pragma unroll
@@ -365,7 +374,7 @@ template <typename T> struct Z8<T, true> {
         w[0] = w[1] = e[0] = e[1] = 0u;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const int at = min(c + k, g.C - 1);
+            const int at = min(c + 16 * k, g.C - 1);
             w[k >> 2] |= (unsigned)((const unsigned char*)g.z)[(long long)m * g.C + at] << (8 * (k & 3));
             e[k >> 2] |= (unsigned)g.exps[(long long)(m >> 5) * g.C + at] << (8 * (k & 3));
         }
@@ -395,7 +404,6 @@ template <typename T, bool ACT8>
 __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* rows, int n, int l, long long piece, bool whole, int block, float* red) {
     const int ncb = (g.C + 127) / 128, cb = block % ncb, j0 = block / ncb * 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-    const int c = cb * 128 + 8 * i;
     if (n == 0) {                                                          // an adapter without rows has one piece: its part of the result is zero
         const int c0 = cb * 128, w = min(128, g.C - c0), nj = min(16, r - j0);
         for (int e = threadIdx.x; e < 128 * 16; e += 256) {
@@ -405,6 +413,7 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
         return;
     }
     const bool vec = Z8<T, ACT8>::aligned(g);
+    const int c = cb * 128 + (vec ? 8 * i : i), cs = vec ? 1 : 16;         // a lane's columns: c, c + cs ..
     const int per = ((n + 3) / 4 + 3) & ~3, r0 = wave * per, r1 = min(r0 + per, n);
     const int j = min(j0 + i, r - 1);
     f32x4 acc[8];
@@ -459,7 +468,7 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
                 for (int t = 0; t < 8; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[s], z[s].get(t), acc[t], 0, 0, 0);
         }
     }
-    // element e of tile t: rank j0 + 4 q + e of column c + t
+    // element e of tile t: rank j0 + 4 q + e of column c + t cs
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
@@ -471,7 +480,7 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
 #pragma unroll
         for (int w = 1; w < 4; ++w) v += red[at + w * 32 * 64];
         if constexpr (B16) {                                           // an infinity of z times the parts of p may be a NaN that their sum's product is not
-            const int jj = j0 + 4 * q + e, cc = c + t;
+            const int jj = j0 + 4 * q + e, cc = c + t * cs;
             if (v != v && jj < r && cc < g.C) {
                 v = 0.f;
 #pragma unroll 4
@@ -484,11 +493,11 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             const int t = 2 * wave + t2, jj = j0 + 4 * q;
-            T* po = (T*)g.out + ((long long)l * g.C + c + t) * r + jj;
+            T* po = (T*)g.out + ((long long)l * g.C + c + t * cs) * r + jj;
             T h[4] __attribute__((aligned(16)));
 #pragma unroll
             for (int e = 0; e < 4; ++e) down(h + e, total(t, e));
-            if (c + t < g.C) {
+            if (c + t * cs < g.C) {
                 if (r % 4 == 0 && ((uintptr_t)g.out & (4 * sizeof(T) - 1)) == 0) {
                     if (jj < r) {
                         if (sizeof(T) == 4) *(uint4*)po = *(const uint4*)h;
@@ -511,13 +520,13 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
                 float* po = g.part + (piece * r + jj) * g.C + c;
 #pragma unroll
                 for (int t = 0; t < 8; ++t)
-                    if (c + t < g.C) po[t] = v[t];
+                    if (c + t * cs < g.C) po[t * cs] = v[t];
             } else {
                 T* po = (T*)g.out + ((long long)l * r + jj) * g.C + c;
                 T h[8] __attribute__((aligned(16)));
 #pragma unroll
                 for (int t = 0; t < 8; ++t) down(h + t, v[t]);
-                if (g.C % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {
+                if (vec && g.C % 8 == 0 && ((uintptr_t)g.out & 15) == 0) {
                     if (c < g.C) {
 #pragma unroll
                         for (int k = 0; k < (int)sizeof(h) / 16; ++k) *((uint4*)po + k) = *((const uint4*)h + k);
@@ -525,7 +534,7 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
                 } else {
 #pragma unroll
                     for (int t = 0; t < 8; ++t)
-                        if (c + t < g.C) po[t] = h[t];
+                        if (c + t * cs < g.C) po[t * cs] = h[t];
                 }
             }
         }
@@ -1326,9 +1335,8 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
     AdArgs<T> g{};
     g.x = x; g.ldx = ldx; g.w = w; g.bias = bias; g.a = a; g.b = b; g.scale = scale; g.ids = ids; g.y = y; g.t = t ? t : (float*)(ws + o.t);
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
-    const int V = 16 / (int)sizeof(T);
-    const bool vec = K % V == 0 && ldx % V == 0 && !off16(x) && !off16(w) && !off16(a);
-    if (M <= kOneRows && (long long)M * r * K * (int)sizeof(T) <= kOneBytes) {
+    const bool vec = K % 4 == 0 && ldx % 4 == 0 && !(((uintptr_t)x | (uintptr_t)w | (uintptr_t)a) & (4 * sizeof(T) - 1));      // load4's; few rows
+    if (M <= kOneRows && (long long)M * r * K * (int)sizeof(T) <= (vec ? kOneBytes : kOneOdd)) {
         g.t = t;
         if (vec) hipLaunchKernelGGL((k_ad_one<T, true>), dim3(blocks_of(N, 8)), dim3(256), 0, st, g);
         else hipLaunchKernelGGL((k_ad_one<T, false>), dim3(blocks_of(N, 8)), dim3(256), 0, st, g);
@@ -1355,7 +1363,7 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
     lo.in = x; lo.ldin = ldx; lo.v = a; lo.ldv = K;
     AdGemm<T> m{};
     m.w = w; m.ldw = K;
-    if (K != Kp || ldx % V || off16(x)) {
+    if (K != Kp || ldx % (16 / (int)sizeof(T)) || off16(x)) {
         pr.copy[pr.ncopy++] = copy_job(x, ws + o.xp, ldx, Kp, 0, 0, 1, M, K, Kp, 0);
         lo.in = ws + o.xp; lo.ldin = Kp;
     }
@@ -1387,8 +1395,7 @@ static int backward_t(const T* dy, const void* x, long long ldx, const unsigned 
     AdGrad ga{}, gb{};
     ga.p = g.u; ga.ldp = r; ga.z = x; ga.exps = exps; ga.out = da; ga.ldz = ldx; ga.C = ga.Cp = K; ga.trans = 0; ga.blocks = blocks_of(K, 128) * blocks_of(r, 16);
     gb.p = t; gb.ldp = r; gb.z = dy; gb.out = db; gb.ldz = N; gb.C = gb.Cp = N; gb.trans = 1; gb.blocks = blocks_of(N, 128) * blocks_of(r, 16);
-    const int V = 16 / (int)sizeof(T);
-    const bool vec = N % V == 0 && !off16(dy);
+    const bool vec = N % 4 == 0;                                           // dy itself is 16-byte aligned
     if (M <= kFewRows) {
         few_split(M, K, N, &g.ksplit, &g.kw);
         g.partial = (float*)(ws + o.partial);
