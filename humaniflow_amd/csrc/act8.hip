@@ -677,16 +677,15 @@ int hmf_bn_backward_act8(const float* g, const signed char* codes, const unsigne
     HMF_LAUNCH_CHECK();
     const long long tiles = ((long long)M + 31) / 32 * ct;
     // A launch of its own for the partial sums costs 3 us and the call's host time another 3; adding them in every wave of the second pass costs their reads.
-    const bool fold = tiles * parts <= kFoldReads;
+    const bool nt = (long long)M * C * 4 > kStreamBytes, fold = !nt && tiles * parts <= kFoldReads;
     if (!fold) {
         hipLaunchKernelGGL(k_bn8_finalize, dim3(C / 4), dim3(256), 0, st, part, parts, M, C, gamma, rstd, g_gamma, g_beta, coef);
         HMF_LAUNCH_CHECK();
     }
     const Bn8Fold f{part, gamma, g_gamma, g_beta, parts};
     const dim3 grid((unsigned)((tiles + 3) / 4)), block(256);
-    const bool nt = (long long)M * C * 4 > kStreamBytes;
 #define HMF_BN8A(GZ, NT, FOLD) hipLaunchKernelGGL((k_bn8_apply<GZ, NT, FOLD>), grid, block, 0, st, g, cd, exps, bits, mean, rstd, coef, gy, gz, M, C, ct, tiles, f)
-    if (gz && nt) HMF_BN8A(true, true, false);                             // never folded: a streamed map has far too many tiles
+    if (gz && nt) HMF_BN8A(true, true, false);
     else if (nt) HMF_BN8A(false, true, false);
     else if (gz && fold) HMF_BN8A(true, false, true);
     else if (gz) HMF_BN8A(true, false, false);

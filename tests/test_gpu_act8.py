@@ -162,6 +162,29 @@ def test_bn_backward(M, C, masked, gz):
     assert torch.equal(again[0], gy) and torch.equal(again[2], gg) and torch.equal(again[3], gb)      # no atomics: bit for bit
 
 
+@pytest.mark.parametrize('gz', [False, True])
+def test_bn_backward_of_few_rows_and_many_channels(gz):
+    """A map over 128 MB whose partial sums are few: 256 rows of 131,136 channels.  Compared in float64 on the device, tolerances as above."""
+    M, C = 256, 131136
+    gen = torch.Generator(device='cuda').manual_seed(5)
+    y = torch.randn(M, C, generator=gen, device='cuda')
+    g = torch.randn(M, C, generator=gen, device='cuda')
+    mean = y.mean(dim=0)
+    rstd = torch.rsqrt(y.var(dim=0, unbiased=False) + 1e-2)
+    gamma = 0.5 + torch.rand(C, generator=gen, device='cuda')
+    ck = act8.pack(y)
+    got = act8.bn_backward(g, ck, None, mean, rstd, gamma, want_gz=gz)
+    assert not gz or torch.equal(got[1], g)
+    xhat = (act8.unpack(ck).double() - mean.double()) * rstd.double()
+    z = g.double()
+    gb, gg = z.sum(0), (z * xhat).sum(0)
+    eg, egx = 12 * EPS * z.abs().sum(0), 12 * EPS * (z * xhat).abs().sum(0)
+    assert ((got[3].double() - gb).abs() <= eg).all() and ((got[2].double() - gg).abs() <= egx).all()
+    ca = (gamma * rstd).double()
+    tol = ca * (8 * EPS * (z.abs() + gb.abs() / M + (xhat * gg).abs() / M) + (eg + xhat.abs() * egx) / M)
+    assert ((got[0].double() - ca * (z - gb / M - xhat * gg / M)).abs() <= tol).all()
+
+
 def test_refusals_on_the_device():
     y, scale, shift, res = _bn_case(64, 64, 0, True)
     ck = act8.pack(y)
