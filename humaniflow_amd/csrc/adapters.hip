@@ -637,7 +637,7 @@ __global__ __launch_bounds__(kPrep) void k_ad_prep(const AdPrep a) {
         for (int mb = m0; mb < m1; mb += 64 * U) {
             int v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = mb + 64 * u + lane < m1 ? a.ids[mb + 64 * u + lane] : -2;
+            for (int u = 0; u < U; ++u) v[u] = a.ids[min(mb + 64 * u + lane, m1 - 1)];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const bool in = mb + 64 * u + lane < m1;
@@ -663,7 +663,7 @@ __global__ __launch_bounds__(kPrep) void k_ad_prep(const AdPrep a) {
         for (int mb = m0; mb < m1; mb += 64 * U) {
             int v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = mb + 64 * u + lane < m1 ? a.ids[mb + 64 * u + lane] : -2;
+            for (int u = 0; u < U; ++u) v[u] = a.ids[min(mb + 64 * u + lane, m1 - 1)];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int m = mb + 64 * u + lane, key = (v[u] < 0 || v[u] >= a.L) ? a.L : v[u];
@@ -688,21 +688,21 @@ __global__ __launch_bounds__(kPrep) void k_ad_prep(const AdPrep a) {
     const T* src = (const T*)c.src + bt * c.sbs;
     T* dst = (T*)c.dst + bt * c.dbs;
     const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    T v[16];                                                                // sixteen elements of a thread in flight
+    T v[16];                                                                // sixteen elements of a thread in flight: no load behind a condition
     if (!c.trans) {                                                         // 256 rows x 64 columns
         const int r0 = ir * 256 + y, cc = ic * 64 + x;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = (r0 + 16 * j < c.R && cc < c.C) ? src[(long long)(r0 + 16 * j) * c.lds_ + cc] : (T)0;
+        for (int j = 0; j < 16; ++j) v[j] = src[(long long)min(r0 + 16 * j, c.R - 1) * c.lds_ + min(cc, c.C - 1)];
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-            if (r0 + 16 * j < c.R && cc < c.Cp) dst[(long long)(r0 + 16 * j) * c.ldd + cc] = v[j];
+            if (r0 + 16 * j < c.R && cc < c.Cp) dst[(long long)(r0 + 16 * j) * c.ldd + cc] = cc < c.C ? v[j] : (T)0;
         return;
     }
     const int r0 = ir * 64, c0 = ic * 256;                                  // 64 rows x 256 columns of the destination
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = (r0 + x < c.R && c0 + y + 16 * j < c.C) ? src[(long long)(c0 + y + 16 * j) * c.lds_ + r0 + x] : (T)0;
+    for (int j = 0; j < 16; ++j) v[j] = src[(long long)min(c0 + y + 16 * j, c.C - 1) * c.lds_ + min(r0 + x, c.R - 1)];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) s[x][y + 16 * j] = v[j];
+    for (int j = 0; j < 16; ++j) s[x][y + 16 * j] = c0 + y + 16 * j < c.C ? v[j] : (T)0;
     __syncthreads();
     const int xc = threadIdx.x & 255, yr = threadIdx.x >> 8;
 #pragma unroll
