@@ -235,6 +235,55 @@ def test_streams_repeats_and_graph_replays():
             assert all(torch.equal(a, b) for a, b in zip(want, held)), (M, k)
 
 
+@pytest.mark.parametrize('checkpoint', [None, 'int8'])
+def test_captured_fit(checkpoint):
+    """Forward and backward through autograd in one graph, replayed between the program's own passes; the kernels add in a fixed order, so the results are the same bits."""
+    c = _case(300, 96, 64, 8, 3, 'mixed', torch.float32, 9)
+    w = torch.randn(300, 64, device='cuda')
+    leaf = {k: c[k].clone().requires_grad_(True) for k in ('x', 'A', 'B')}
+
+    def step():
+        y = adapters.adapted_linear(**{**c, **leaf}, checkpoint=checkpoint)
+        return [y.detach(), *torch.autograd.grad((y * w).sum(), list(leaf.values()))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(3):
+        with torch.no_grad():
+            leaf['x'].mul_(0.8)
+            leaf['A'].add_(0.01)
+        c['ids'].copy_(torch.randint(-1, 3, (300,), device='cuda'))
+        want = [t.clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, held)), k
+
+
+def test_capture_beside_a_living_eager_pass_is_refused(monkeypatch):
+    """The check itself, without a capture: a pass over the same leaves on the default stream is alive, then it is not."""
+    c = _case(8, 64, 48, 4, 2, 'mixed', torch.float32, 0)
+    leaf = {k: c[k].clone().requires_grad_(True) for k in ('A', 'B')}
+    y = adapters.adapted_linear(**{**c, **leaf})
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    with pytest.raises(RuntimeError, match='still alive'):
+        adapters.adapted_linear(**{**c, **leaf})
+    del y
+    adapters.adapted_linear(**{**c, **leaf}).sum().backward()
+    monkeypatch.undo()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = adapters.adapted_linear(**{**c, **leaf})
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    adapters.adapted_linear(**{**c, **leaf})
+    torch.cuda.current_stream().wait_stream(side)
+
+
 # ---- the model's heads ----------------------------------------------------------------------------------------------------------
 def _model(layers=18):
     cfg = H.get_humaniflow_cfg_defaults()
