@@ -105,17 +105,16 @@ __global__ __launch_bounds__(256) void k_act8_pack(const void* __restrict__ x, l
     Row<BF16> r[8];
     bool in[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8; ++i) {                                     // what is not there reads the last row (of this block) or column: no load behind a condition
         in[i] = live && m0 + 4 * i < M;
-        if (in[i]) r[i].load(x, (long long)(m0 + 4 * i) * ld + c);
+        r[i].load(x, (long long)min(m0 + 4 * i, M - 1) * ld + min(c, C - V));
     }
     unsigned int top[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         top[k] = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (in[i]) top[k] = max(top[k], fin_mag(r[i].get(k)));
+        for (int i = 0; i < 8; ++i) top[k] = max(top[k], fin_mag(r[i].get(k)));
     }
     float inv[V];
     unsigned int E[V];
@@ -189,11 +188,8 @@ __global__ __launch_bounds__(256) void k_act8_pack_any(const void* __restrict__ 
     float v[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-        v[i] = 0.f;
-        if (i < n) {
-            const long long o = (long long)(m0 + i) * ld + c;
-            v[i] = BF16 ? bf16_to_f32(((const unsigned short*)x)[o]) : ((const float*)x)[o];
-        }
+        const long long o = (long long)(m0 + min(i, n - 1)) * ld + c;
+        v[i] = BF16 ? bf16_to_f32(((const unsigned short*)x)[o]) : ((const float*)x)[o];
     }
     unsigned int top = 0u;
 #pragma unroll
@@ -325,8 +321,7 @@ __global__ __launch_bounds__(256) void k_act8_restore(const unsigned char* __res
     const float floor_ = bits ? 0.f : -INFINITY;
     unsigned int w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (m0 + 4 * i < M) w[i] = *(const unsigned int*)(codes + (long long)(m0 + 4 * i) * C + c);
+    for (int i = 0; i < 8; ++i) w[i] = *(const unsigned int*)(codes + (long long)min(m0 + 4 * i, M - 1) * C + c);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (m0 + 4 * i < M) {
