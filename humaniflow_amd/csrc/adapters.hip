@@ -1292,7 +1292,7 @@ static int check_sizes(const char* who, int M, int K, int N, int r, int L) {
     // a grid has under 2^32 threads in a dimension, and its y extent is 16 bits
     const long long c = std::max(K, N) + 128ll, tc = c / 64 + 1, most = 4194303;                      // work-groups of 1,024
     const bool few = M <= kFewRows;
-    if (L > 65535 || (long long)L + M / kFewRows > 65535 || (few && M * c > 0xffffff00ll) ||
+    if (L > 65535 || (long long)L + M / kFewRows > 65535 || (few && (M * c > 0xffffff00ll || L * (c / 128 + 1) * (r / 16 + 1) > 4 * most - c)) ||
         (!few && (long long)L + 1 + (M / 64 + 1) * tc + (N / 64 + 1) * (long long)(K / 64 + 3) + std::max((long long)L * r / 64 + 1, (long long)L) * tc > most))
         return fail(HMF_ERR_UNSUPPORTED, "%s: M=%d K=%d N=%d r=%d L=%d exceed the grid", who, M, K, N, r, L);
     return HMF_OK;

@@ -69,6 +69,7 @@ def test_refusals_of_the_c_entry_points(lib):
     bw = lambda dy=p, ldx=6, exps=n, M=4, r=2, ws=p, nb=1 << 20: lib.hmf_adapted_linear_backward(dy, p, ldx, exps, p, p, p, p, p, p, M, 6, 3, r, 2, 0, p, p, p, ws, nb, n)
     assert bw(dy=n) == -1 and bw(ldx=5) == -1 and bw(ldx=7, exps=p) == -1 and bw(M=0) == -1 and bw(r=65) == -2 and bw(nb=need - 1) == -4 and bw(ws=n) == -4
     assert lib.hmf_adapted_linear_workspace_bytes(0, 6, 3, 2, 2, 0) == 0
+    assert fw(L=65535, N=1 << 17) == -2 and b'grid' in lib.hmf_last_error()      # a work-group of the gradients per adapter and 128 columns
 
 
 def test_module_layout_and_refusals():
