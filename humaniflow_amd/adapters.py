@@ -86,9 +86,9 @@ def adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t=True):
     lib = _lib.load()
     bf16 = int(weight.dtype == torch.bfloat16)
     n = lib.hmf_adapted_linear_workspace_bytes(M, K, N, r, L, bf16)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None      # a few rows need none
     _lib.check(lib.hmf_adapted_linear(x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(),
-                                      ids.data_ptr(), M, K, N, r, L, bf16, y.data_ptr(), None if t is None else t.data_ptr(), ws.data_ptr(), n, st), 'hmf_adapted_linear')
+                                      ids.data_ptr(), M, K, N, r, L, bf16, y.data_ptr(), None if t is None else t.data_ptr(), None if ws is None else ws.data_ptr(), n, st), 'hmf_adapted_linear')
     return y, t
 
 

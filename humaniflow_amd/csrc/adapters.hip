@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void k_ad_few(const AdArgs<T> a, int tiles_o, 
 
 // One to four rows (a single image): everything in ONE launch, since a second one costs as much as the work.  A work-group finds the rows' t itself -- A_l is read once per
 // work-group, from L2 -- and then its waves two outputs each, lanes along K.  1 row, 2,048 -> 1,024, rank 16 in 32 bits: 7.6 us, and two launches of 9 us in all in the form below.
-constexpr int kOneRows = 4, kOneBytes = 512 << 10, kOneOdd = 64 << 10;      // rows; bytes of A that a work-group reads for them, and where its rows are not aligned (4 rows, 1,941 ->
+constexpr int kOneRows = 4, kOneBytes = 512 << 10, kOneOdd = 64 << 10;      // rows; bytes of A that a work-group reads for them, and where its rows are not multiples of 4 (4 rows, 1,941 ->
 // 1,379, rank 15: 56 us, 18 below; 4 rows, 1,001 -> 64, rank 8, bfloat16: 16 us, 18 below)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_ad_one(const AdArgs<T> a) {
@@ -1239,10 +1239,15 @@ static size_t gemm_partial(int M, int O, int Cp, size_t z) {
 // the many-row form's rows: whole chunks of 128 bytes, 16-byte aligned
 static inline int padded(int C, size_t z) { const int bk = (int)(128 / z); return (C + bk - 1) / bk * bk; }
 static inline int rank_pitch(int r) { return (r + 3) & ~3; }
+// one launch for one to four rows: a rule on the sizes alone, so that its callers need no workspace (an allocation is 1.3 us of 12)
+static inline bool one_launch(int M, int K, int r, size_t z) {
+    return M <= kOneRows && (long long)M * r * K * (int)z <= (K % 4 == 0 ? kOneBytes : kOneOdd);
+}
 struct FwdWs { size_t t, partial, order, key, seg, xp, wp, ap, total; };
 static FwdWs fwd_ws(int M, int K, int N, int r, int L, size_t z) {
     FwdWs w{};
     size_t o = 0;
+    if (one_launch(M, K, r, z)) return w;
     w.t = o; o += al((size_t)M * rank_pitch(r) * 4);
     if (M <= kFewRows) {
         int ks, kw;
@@ -1336,7 +1341,7 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
     g.x = x; g.ldx = ldx; g.w = w; g.bias = bias; g.a = a; g.b = b; g.scale = scale; g.ids = ids; g.y = y; g.t = t ? t : (float*)(ws + o.t);
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
     const bool vec = K % 4 == 0 && ldx % 4 == 0 && !(((uintptr_t)x | (uintptr_t)w | (uintptr_t)a) & (4 * sizeof(T) - 1));      // load4's; few rows
-    if (M <= kOneRows && (long long)M * r * K * (int)sizeof(T) <= (vec ? kOneBytes : kOneOdd)) {
+    if (one_launch(M, K, r, sizeof(T))) {
         g.t = t;
         if (vec) hipLaunchKernelGGL((k_ad_one<T, true>), dim3(blocks_of(N, 8)), dim3(256), 0, st, g);
         else hipLaunchKernelGGL((k_ad_one<T, false>), dim3(blocks_of(N, 8)), dim3(256), 0, st, g);
@@ -1465,7 +1470,7 @@ int hmf_adapted_linear(const void* x, long long ldx, const void* w, const void* 
     if (M == 0) return HMF_OK;
     if (!x || !w || !a || !b || !scale || !ids || !y || ldx < K) return fail(HMF_ERR_INVALID, "hmf_adapted_linear: null argument or ldx=%lld < K=%d", ldx, K);
     const size_t need = fwd_ws(M, K, N, r, L, bf16 ? 2 : 4).total;
-    if (!workspace || workspace_bytes < need || off16(workspace))
+    if (need && (!workspace || workspace_bytes < need || off16(workspace)))
         return fail(HMF_ERR_WORKSPACE, "hmf_adapted_linear: workspace %zu < %zu bytes (16-byte aligned)", workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;
     if (bf16)

@@ -58,8 +58,9 @@ def test_refusals_of_the_c_entry_points(lib):
     buf = (C.c_float * 4096)()
     p = C.c_void_p((C.addressof(buf) + 15) & ~15)
     n = C.c_void_p(None)
-    need = lib.hmf_adapted_linear_workspace_bytes(4, 6, 3, 2, 2, 0)
-    fw = lambda x=p, ldx=6, M=4, K=6, N=3, r=2, L=2, ws=p, nb=1 << 20: lib.hmf_adapted_linear(x, ldx, p, n, p, p, p, p, M, K, N, r, L, 0, p, n, ws, nb, n)
+    need = lib.hmf_adapted_linear_workspace_bytes(5, 6, 3, 2, 2, 0)
+    assert lib.hmf_adapted_linear_workspace_bytes(4, 6, 3, 2, 2, 0) == 0      # one launch
+    fw = lambda x=p, ldx=6, M=5, K=6, N=3, r=2, L=2, ws=p, nb=1 << 20: lib.hmf_adapted_linear(x, ldx, p, n, p, p, p, p, M, K, N, r, L, 0, p, n, ws, nb, n)
     assert need > 0 and fw(M=0) == 0
     assert fw(x=n) == -1 and fw(ldx=5) == -1 and fw(K=0) == -1 and fw(M=-1) == -1 and fw(L=0) == -1 and fw(r=0) == -1
     assert fw(r=65) == -2 and fw(L=70000) == -2
