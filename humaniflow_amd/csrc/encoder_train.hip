@@ -83,7 +83,9 @@ __global__ __launch_bounds__(256) void k_bn_apply(const f32x4* __restrict__ y, c
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256) {
         const int c = (int)(i % C4) * 4;
         const f32x4 sc = *(const f32x4*)(scale + c), sh = *(const f32x4*)(shift + c);
-        f32x4 v = y[i] * sc + sh;
+        f32x4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = fmaf(y[i][k], sc[k], sh[k]);      // one rounding, written out: act8.hip's form of this unit has the same bits
         if (res) v += res[i];
         if (relu) {                                    // NaN-propagating, like torch.relu (fmaxf alone would turn a NaN into 0 and hide it from nan_policy='rollback')
 #pragma unroll
