@@ -60,6 +60,8 @@ __device__ __forceinline__ float wave_sum(float v) {
     for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
     return v;
 }
+__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+__device__ __forceinline__ bool finite(bf16_t v) { return (v & 0x7f80u) != 0x7f80u; }
 __device__ __forceinline__ float nan32() { return __uint_as_float(0x7fc00000u); }
 
 template <typename T> struct AdArgs {
@@ -479,9 +481,9 @@ __device__ __forceinline__ void grad_piece(const AdGrad& g, int r, const int* ro
         float v = red[at];
 #pragma unroll
         for (int w = 1; w < 4; ++w) v += red[at + w * 32 * 64];
-        if constexpr (B16) {                                           // an infinity of z times the parts of p may be a NaN that their sum's product is not
-            const int jj = j0 + 4 * q + e, cc = c + t * cs;
-            if (v != v && jj < r && cc < g.C) {
+        if constexpr (B16) {                                           // an infinity of z times the parts of p may be a NaN, and a p near the largest float's first
+            const int jj = j0 + 4 * q + e, cc = c + t * cs;            // part an infinity, where their own product is neither
+            if (!finite(v) && jj < r && cc < g.C) {
                 v = 0.f;
 #pragma unroll 4
                 for (int k = 0; k < n; ++k) v = fmaf(g.p[(long long)rows[k] * g.ldp + jj], Z8<T, ACT8>::one(g, rows[k], cc), v);
@@ -736,8 +738,6 @@ template <> struct Mma<bf16_t> {
     }
     static __device__ __forceinline__ bf16_t part(float v, int lo) { return to_bf16(lo ? bf16_left(v) : v); }      // high half, and what it leaves
 };
-__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
-__device__ __forceinline__ bool finite(bf16_t v) { return (v & 0x7f80u) != 0x7f80u; }
 
 // Piece z of the order: segment l (of n) has max(MIN, ceil(rows / R)) pieces of R rows, one behind the other.  All lanes of a wave return the same: the segment, how many
 // pieces it has, this one's first place and its end; l = n: no such piece.
@@ -871,7 +871,8 @@ template <typename T> struct AdGemm {
 // per CU, one's start and end under the other's products) where it has more.
 // After the shared weight's chunks come the adapters': 16-byte piece P of a row belongs to the tile's adapter list[P / pp] and holds E of its ranks (bfloat16: the
 // high halves of all ranks, then the low ones).  The rows of other adapters hold zeros there,
-// and a zero times an infinity or a NaN of a weight would reach them: such weights are staged as zeros and added to their own rows at the end.
+// and a zero times an infinity or a NaN of a weight would reach them: such weights are staged as zeros and added to their own rows at the end, and so are values of low
+// that are not finite or, in bfloat16, become infinite there (from 3.39e38 on).
 template <typename T, int BT, int RB>
 __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
     typedef Mma<T> X;
@@ -983,12 +984,15 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
                 zw[k] = out && ej0 + k < a.r ? ew[s][k] : (T)0;
                 ok &= finite(zw[k]);
                 zx[k] = X::part(mine && ej0 + k < a.r ? ex[s][k / 4][k & 3] : 0.f, elo);
+                ok &= finite(zx[k]);
             }
             if (!ok) {
                 *odd = 1;
 #pragma unroll
-                for (int k = 0; k < E; ++k)
+                for (int k = 0; k < E; ++k) {
                     if (!finite(zw[k])) zw[k] = 0;
+                    if (!finite(zx[k])) zx[k] = 0;
+                }
             }
             *(frag*)(smem + st * STAGE + at) = zw;
             *(frag*)(smem + st * STAGE + OP + at) = zx;
@@ -1126,7 +1130,8 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
                     else if (id >= 0 && o + k < a.O)
                         for (int j = 0; j < a.r; ++j) {
                             const T vv = a.v[id * a.vl + (o + k) * a.vo + j * a.vj];
-                            if (!finite(vv)) z[k] = fmaf(a.low[(long long)m * a.rp + j], up(vv), z[k]);
+                            const float lv = a.low[(long long)m * a.rp + j];
+                            if (!finite(vv) || !finite(X::part(lv, 0))) z[k] = fmaf(lv, up(vv), z[k]);
                         }
                 }
             }
