@@ -14,6 +14,7 @@ import torch
 from torch import nn
 
 from . import _lib, act8
+from .autograd import refuse_capture_beside_default_stream_pass
 
 MAX_RANK = 64
 
@@ -148,19 +149,6 @@ class _AdaptedLinear(torch.autograd.Function):
         return dx, None, None, dA, dB, None, None, None
 
 
-def _leaves_may_be_captured(y):
-    """A leaf's gradient is added on the stream on which its first living graph was built.  If that is the legacy default stream and this graph is being captured into
-    a HIP graph, the captured backward pass would have to wait for a stream that no capture can hold, which ends the process: refused here instead."""
-    capturing = torch.cuda.is_current_stream_capturing()
-    for node, _ in y.grad_fn.next_functions:
-        if hasattr(node, 'variable'):                                      # a leaf's; what is noted lives as long as a graph of the leaf does
-            if not capturing:
-                node.metadata.setdefault('hmf_stream', torch._C._cuda_getCurrentRawStream(y.device.index))
-            elif node.metadata.get('hmf_stream') == 0:
-                raise RuntimeError('humaniflow_amd: adapted_linear is captured while a pass over the same parameters, run eagerly on the default stream, is still '
-                                   'alive: let go of its outputs and loss first (del), or run it on another stream')
-
-
 def adapted_linear(x, weight, bias, A, B, scale, ids, checkpoint=None):
     """y (M, N).  Differentiable w.r.t. x, A and B; the shared projection is held fixed (a weight, bias or scale that requires a gradient is refused).
     checkpoint='int8': the backward pass keeps x in 8 bits.  To capture forward and backward into a HIP graph, first let go of every eager pass over the same
@@ -172,7 +160,7 @@ def adapted_linear(x, weight, bias, A, B, scale, ids, checkpoint=None):
             raise RuntimeError('humaniflow_amd: adapters are fitted beside a fixed projection: call requires_grad_(False) on its weight and bias, and on scale')
         if x.requires_grad or A.requires_grad or B.requires_grad:
             y = _AdaptedLinear.apply(x, weight, bias, A, B, scale, ids, checkpoint)
-            _leaves_may_be_captured(y)
+            refuse_capture_beside_default_stream_pass([n for n, _ in y.grad_fn.next_functions if hasattr(n, 'variable')], y.device, 'adapted_linear')
             return y
     return adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t=False)[0]
 

@@ -36,6 +36,19 @@ def _atb(A, B, batch, rows, m, n, lda, ldb, sA, sB, want_sum):
     return Cm, sm
 
 
+def refuse_capture_beside_default_stream_pass(nodes, device, what):
+    """A leaf's gradient is added on the stream on which its first living graph was built.  If that is the legacy default stream and this graph is being captured into
+    a HIP graph, the captured backward pass would have to wait for a stream that no capture can hold, which ends the process: refused here instead.
+    nodes: the leaves' nodes in the graph just built; what is noted on one lives as long as a graph of its leaf does."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    for node in nodes:
+        if not capturing:
+            node.metadata.setdefault('hmf_stream', torch._C._cuda_getCurrentRawStream(device.index))
+        elif node.metadata.get('hmf_stream') == 0:
+            raise RuntimeError('humaniflow_amd: %s is captured while a pass over the same parameters, run eagerly on the default stream, is still '
+                               'alive: let go of its outputs and loss first (del), or run it on another stream' % what)
+
+
 # ---- records of the flow backward kernels ---------------------------------------------------------------------------------
 class _Records:
     """Device buffers for hmf_flow_grad_records_t: part-major [P][2][rows][width]."""
