@@ -712,6 +712,14 @@ __global__ __launch_bounds__(kPrep) void k_ad_prep(const AdPrep a) {
         if (r0 + yr + 4 * j < c.R && c0 + xc < c.Cp) dst[(long long)(r0 + yr + 4 * j) * c.ldd + c0 + xc] = s[yr + 4 * j][xc];
 }
 
+// Whether any of the 16 bytes of u and v holds an exponent of all ones: an infinity or a NaN.  ONES: the exponents' bits in a word, LOW: their lowest ones, which added to
+// an exponent of all ones carry into the sign's place and no further.
+template <unsigned ONES, unsigned LOW, typename F> __device__ __forceinline__ bool odd16(F u, F v) {
+    const uint4 a = __builtin_bit_cast(uint4, u), b = __builtin_bit_cast(uint4, v);
+    const unsigned s = ((a.x & ONES) + LOW) | ((a.y & ONES) + LOW) | ((a.z & ONES) + LOW) | ((a.w & ONES) + LOW) | ((b.x & ONES) + LOW) | ((b.y & ONES) + LOW) |
+                       ((b.z & ONES) + LOW) | ((b.w & ONES) + LOW);
+    return (s & (ONES + LOW)) != 0u;
+}
 // What the two types differ in.  A fragment is 16 bytes of a row in both.
 template <typename T> struct Mma;
 template <> struct Mma<float> {
@@ -726,6 +734,7 @@ template <> struct Mma<float> {
         return c;
     }
     static __device__ __forceinline__ float part(float v, int) { return v; }
+    static __device__ __forceinline__ bool any_odd(frag u, frag v) { return odd16<0x7f800000u, 0x00800000u>(u, v); }
 };
 template <> struct Mma<bf16_t> {
     static constexpr int E = 8, HL = 2, STEPS = 1;
@@ -737,6 +746,7 @@ template <> struct Mma<bf16_t> {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ bf16_t part(float v, int lo) { return to_bf16(lo ? bf16_left(v) : v); }      // high half, and what it leaves
+    static __device__ __forceinline__ bool any_odd(frag u, frag v) { return odd16<0x7f807f80u, 0x00800080u>(u, v); }
 };
 
 // Piece z of the order: segment l (of n) has max(MIN, ceil(rows / R)) pieces of R rows, one behind the other.  All lanes of a wave return the same: the segment, how many
@@ -978,15 +988,12 @@ __global__ __launch_bounds__(256) void k_ad_gemm(const AdGemm<T> a) {
             const int e = tid + 256 * s, row = e / PR, at = row * RB + ((e % PR) ^ swizzle(row)) * 16;
             const bool mine = elive && slot[row] == ead, out = elive && o0 + row < a.O;
             frag zw, zx;
-            bool ok = true;
 #pragma unroll
             for (int k = 0; k < E; ++k) {
                 zw[k] = out && ej0 + k < a.r ? ew[s][k] : (T)0;
-                ok &= finite(zw[k]);
                 zx[k] = X::part(mine && ej0 + k < a.r ? ex[s][k / 4][k & 3] : 0.f, elo);
-                ok &= finite(zx[k]);
             }
-            if (!ok) {
+            if (X::any_odd(zw, zx)) {
                 *odd = 1;
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
