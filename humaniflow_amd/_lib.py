@@ -95,8 +95,10 @@ _SIGS = {
     'hmf_heads_train': (C.c_int, [_VP, C.c_int, C.c_int, _VP, _VP, C.c_int] + [_VP] * 8 + [C.c_int] + [_VP] * 8 + [C.c_size_t, _VP]),
     'hmf_heads_backward': (C.c_int, [_VP, _VP, C.c_int, C.c_int, C.c_int] + [_VP] * 16),
     'hmf_adapted_linear_workspace_bytes': (C.c_size_t, [C.c_int] * 6),
+    'hmf_adapted_linear_workspace_bytes_for': (C.c_size_t, [_VP, C.c_longlong, _VP, _VP] + [C.c_int] * 6),
     'hmf_adapted_linear': (C.c_int, [_VP, C.c_longlong] + [_VP] * 6 + [C.c_int] * 6 + [_VP, _VP, _VP, C.c_size_t, _VP]),
     'hmf_adapted_linear_backward_workspace_bytes': (C.c_size_t, [C.c_int] * 6),
+    'hmf_adapted_linear_backward_workspace_bytes_for': (C.c_size_t, [C.c_int] * 7),
     'hmf_adapted_linear_backward': (C.c_int, [_VP, _VP, C.c_longlong] + [_VP] * 7 + [C.c_int] * 6 + [_VP] * 4 + [C.c_size_t, _VP]),
     'hmf_flow_isgc': (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, _VP, _VP]),
     'hmf_flow_isgc_train': (C.c_int, [_VP] * 7 + [C.c_int, C.c_int, _VP, _VP, _VP]),

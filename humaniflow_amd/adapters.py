@@ -86,7 +86,7 @@ def adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t=True):
     t = torch.empty((M, r), dtype=torch.float32, device=dev) if need_t else None
     lib = _lib.load()
     bf16 = int(weight.dtype == torch.bfloat16)
-    n = lib.hmf_adapted_linear_workspace_bytes(M, K, N, r, L, bf16)
+    n = lib.hmf_adapted_linear_workspace_bytes_for(x.data_ptr(), ldx, weight.data_ptr(), A.data_ptr(), M, K, N, r, L, bf16)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None      # a few rows need none
     _lib.check(lib.hmf_adapted_linear(x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(),
                                       ids.data_ptr(), M, K, N, r, L, bf16, y.data_ptr(), None if t is None else t.data_ptr(), None if ws is None else ws.data_ptr(), n, st), 'hmf_adapted_linear')
@@ -123,7 +123,7 @@ def adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=True):
     dA, dB = torch.empty_like(A), torch.empty_like(B)
     lib = _lib.load()
     bf16 = int(dt == torch.bfloat16)
-    n = lib.hmf_adapted_linear_backward_workspace_bytes(M, K, N, r, L, bf16)
+    n = lib.hmf_adapted_linear_backward_workspace_bytes_for(M, K, N, r, L, bf16, int(need_dx))
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     _lib.check(lib.hmf_adapted_linear_backward(dy.data_ptr(), xp, ldx, exps, t.data_ptr(), weight.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(), ids.data_ptr(),
                                                M, K, N, r, L, bf16, None if dx is None else dx.data_ptr(), dA.data_ptr(), dB.data_ptr(), ws.data_ptr(), n, st),

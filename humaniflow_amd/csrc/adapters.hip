@@ -333,7 +333,7 @@ struct AdGrad {
     const void* z;                     // rows of pitch ldz, or the codes (M, C)
     const unsigned char* exps;         // with codes
     void* out;                         // (L, r, C), or (L, C, r) with trans
-    float* part;                       // [pieces][r][C]
+    float* part;                       // [pieces of adapters that have several][r][C]
     long long ldz, ldp;
     int C, Cp, trans, blocks;          // columns, columns that may be read; blocks: blocks of 128 columns x 16 ranks, columns first
 };
@@ -750,11 +750,11 @@ template <> struct Mma<bf16_t> {
 };
 
 // Piece z of the order: segment l (of n) has max(MIN, ceil(rows / R)) pieces of R rows, one behind the other.  All lanes of a wave return the same: the segment, how many
-// pieces it has, this one's first place and its end; l = n: no such piece.
-template <int R, int MIN>
-__device__ __forceinline__ void find_piece(const int* seg, int n, int z, int& l, int& np, int& at, int& end) {
+// pieces it has, this one's first place and its end; l = n: no such piece.  PART: and `part`, its number among the pieces of segments that have several.
+template <int R, int MIN, bool PART>
+__device__ __forceinline__ void find_piece(const int* seg, int n, int z, int& l, int& np, int& at, int& end, int& part) {
     const int lane = threadIdx.x & 63;
-    int base = 0;
+    int base = 0, pbase = 0;
     for (int l0 = 0; l0 < n; l0 += 64) {
         const int li = l0 + lane;
         const int s0 = seg[min(li, n)], s1 = seg[min(li + 1, n)], rows = s1 - s0;
@@ -766,18 +766,26 @@ __device__ __forceinline__ void find_piece(const int* seg, int n, int z, int& l,
             if (lane >= d) incl += o;
         }
         const unsigned long long over = __ballot(base + incl > z);
+        const int k = over ? __ffsll((long long)over) - 1 : 64;              // the piece's segment in these 64
+        if (PART) {
+            int before = lane < k && mine > 1 ? mine : 0;
+#pragma unroll
+            for (int d = 32; d >= 1; d >>= 1) before += __shfl_xor(before, d);
+            pbase += before;
+        }
         if (over) {
-            const int k = __ffsll((long long)over) - 1;
             l = l0 + k;
             np = __shfl(mine, k);
-            at = __shfl(s0, k) + (z - (base + __shfl(incl, k) - np)) * R;
+            const int nth = z - (base + __shfl(incl, k) - np);
+            at = __shfl(s0, k) + nth * R;
             end = min(at + R, __shfl(s1, k));
+            part = pbase + nth;
             return;
         }
         base += __shfl(incl, 63);
     }
     l = n;
-    np = at = end = 0;
+    np = at = end = part = 0;
 }
 
 typedef __attribute__((address_space(3))) void* ad_lds_t;
@@ -806,8 +814,8 @@ __global__ __launch_bounds__(1024) void k_ad_low(const AdLow a) {
     __shared__ __attribute__((aligned(16))) char smem[16 * 2 * U * 1024];
     float* red = (float*)smem;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, q = lane >> 4;
-    int ad, np, first, end;
-    find_piece<16, 0>(a.seg, a.L + 1, blockIdx.x, ad, np, first, end);      // the rows without an adapter are the last segment
+    int ad, np, first, end, part;
+    find_piece<16, 0, false>(a.seg, a.L + 1, blockIdx.x, ad, np, first, end, part);      // the rows without an adapter are the last segment
     if (ad > a.L) return;
     ad = __builtin_amdgcn_readfirstlane(ad);
     const bool live = first + i < end;
@@ -1178,15 +1186,15 @@ template <typename T, bool ACT8>
 __global__ __launch_bounds__(256) void k_ad_grads(const AdGrad da, const AdGrad db, const int* __restrict__ order, const int* __restrict__ seg, int r, int L) {
     __shared__ float red[kGradLds];
     __shared__ int rows[kFewRows];
-    int l, np, s0, end;
-    find_piece<kFewRows, 1>(seg, L, blockIdx.y, l, np, s0, end);
+    int l, np, s0, end, part;
+    find_piece<kFewRows, 1, true>(seg, L, blockIdx.y, l, np, s0, end, part);
     if (l >= L) return;
     const int n = end - s0;
     if ((int)threadIdx.x < n) rows[threadIdx.x] = order[s0 + threadIdx.x];
     __syncthreads();
     const int cb = blockIdx.x;
-    if (cb < da.blocks) grad_piece<T, ACT8>(da, r, rows, n, l, blockIdx.y, np == 1, cb, red);
-    else grad_piece<T, false>(db, r, rows, n, l, blockIdx.y, np == 1, cb - da.blocks, red);
+    if (cb < da.blocks) grad_piece<T, ACT8>(da, r, rows, n, l, part, np == 1, cb, red);
+    else grad_piece<T, false>(db, r, rows, n, l, part, np == 1, cb - da.blocks, red);
 }
 
 // sums of the adapters that had several pieces, in the pieces' order; a column of work-groups per adapter, gone at once where there is nothing to add
@@ -1195,10 +1203,10 @@ __global__ __launch_bounds__(256) void k_ad_grad_join(const AdGrad da, const AdG
     const int l = blockIdx.y, mine = seg[l + 1] - seg[l];
     if (mine <= kFewRows) return;
     const int lane = threadIdx.x & 63, np = (mine + kFewRows - 1) / kFewRows;
-    int first = 0;                                                         // pieces in front of this adapter's
+    int first = 0;                                                         // pieces in front of this adapter's, of adapters that have several
     for (int l0 = 0; l0 < l; l0 += 64) {
-        const int li = l0 + lane;
-        int v = li < l ? max(1, (seg[li + 1] - seg[li] + kFewRows - 1) / kFewRows) : 0;
+        const int li = l0 + lane, rows = li < l ? seg[li + 1] - seg[li] : 0;
+        int v = rows > kFewRows ? (rows + kFewRows - 1) / kFewRows : 0;
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
         first += v;
@@ -1255,8 +1263,15 @@ static inline int rank_pitch(int r) { return (r + 3) & ~3; }
 static inline bool one_launch(int M, int K, int r, size_t z) {
     return M <= kOneRows && (long long)M * r * K * (int)z <= (K % 4 == 0 ? kOneBytes : kOneOdd);
 }
+// how the forward's operands lie: which of them the many-row form has to copy into whole chunks of aligned rows
+struct FwdLayout { bool x, w, a; };
+constexpr FwdLayout kAnyLayout{true, true, true};
+static FwdLayout fwd_layout(const void* x, long long ldx, const void* w, const void* a, int K, size_t z) {
+    const bool odd = K != padded(K, z);
+    return {odd || ldx % (long long)(16 / z) != 0 || off16(x), odd || off16(w), odd || off16(a)};
+}
 struct FwdWs { size_t t, partial, order, key, seg, xp, wp, ap, total; };
-static FwdWs fwd_ws(int M, int K, int N, int r, int L, size_t z) {
+static FwdWs fwd_ws(int M, int K, int N, int r, int L, size_t z, const FwdLayout& copy) {
     FwdWs w{};
     size_t o = 0;
     if (one_launch(M, K, r, z)) return w;
@@ -1270,32 +1285,33 @@ static FwdWs fwd_ws(int M, int K, int N, int r, int L, size_t z) {
         w.order = o; o += al((size_t)M * 4);
         w.key = o; o += al((size_t)M * 4);
         w.seg = o; o += al((size_t)(L + 2) * 4);
-        w.xp = o; o += al(M * Kp * z);                                     // used where x, W or A is not laid out like that
-        w.wp = o; o += al(N * Kp * z);
-        w.ap = o; o += al((size_t)L * r * Kp * z);
+        w.xp = o; o += copy.x ? al(M * Kp * z) : 0;
+        w.wp = o; o += copy.w ? al(N * Kp * z) : 0;
+        w.ap = o; o += copy.a ? al((size_t)L * r * Kp * z) : 0;
         w.partial = o; o += al(gemm_partial(M, N, (int)Kp, z));
     }
     w.total = o;
     return w;
 }
 struct BwdWs { size_t u, partial, order, key, seg, wt, bt, dyp, part_a, part_b, total; };
-static BwdWs bwd_ws(int M, int K, int N, int r, int L, size_t z) {
+static BwdWs bwd_ws(int M, int K, int N, int r, int L, size_t z, bool dx) {
     BwdWs w{};
     size_t o = 0;
     w.u = o; o += al((size_t)M * rank_pitch(r) * 4);
     if (M <= kFewRows) {
         int ks, kw;
         few_split(M, K, N, &ks, &kw);
-        w.partial = o; o += al((size_t)ks * M * K * 4);
+        w.partial = o; o += dx ? al((size_t)ks * M * K * 4) : 0;
     } else {
-        const size_t pieces = (size_t)L + M / kFewRows, Np = padded(N, z);
+        // adapters of several pieces have over kFewRows rows each, and less than one piece each beyond their rows'
+        const size_t pieces = (size_t)std::min(L, M / (kFewRows + 1)) + M / kFewRows, Np = padded(N, z);
         w.order = o; o += al((size_t)M * 4);
         w.key = o; o += al((size_t)M * 4);
         w.seg = o; o += al((size_t)(L + 2) * 4);
-        w.wt = o; o += al(K * Np * z);
+        w.wt = o; o += dx ? al(K * Np * z) : 0;
         w.bt = o; o += al((size_t)L * r * Np * z);
         w.dyp = o; o += N == (int)Np ? 0 : al(M * Np * z);
-        w.partial = o; o += al(gemm_partial(M, K, (int)Np, z));
+        w.partial = o; o += dx ? al(gemm_partial(M, K, (int)Np, z)) : 0;
         w.part_a = o; o += al(pieces * r * K * 4);
         w.part_b = o; o += al(pieces * r * N * 4);
     }
@@ -1348,7 +1364,8 @@ template <typename T> static int gemm(AdGemm<T>& m, void* partial, hipStream_t s
 template <typename T>
 static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const T* a, const T* b, const float* scale, const int* ids, int M, int K, int N, int r, int L,
                      T* y, float* t, char* ws, hipStream_t st) {
-    const FwdWs o = fwd_ws(M, K, N, r, L, sizeof(T));
+    const FwdLayout copy = fwd_layout(x, ldx, w, a, K, sizeof(T));
+    const FwdWs o = fwd_ws(M, K, N, r, L, sizeof(T), copy);
     AdArgs<T> g{};
     g.x = x; g.ldx = ldx; g.w = w; g.bias = bias; g.a = a; g.b = b; g.scale = scale; g.ids = ids; g.y = y; g.t = t ? t : (float*)(ws + o.t);
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
@@ -1380,15 +1397,15 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
     lo.in = x; lo.ldin = ldx; lo.v = a; lo.ldv = K;
     AdGemm<T> m{};
     m.w = w; m.ldw = K;
-    if (K != Kp || ldx % (16 / (int)sizeof(T)) || off16(x)) {
+    if (copy.x) {
         pr.copy[pr.ncopy++] = copy_job(x, ws + o.xp, ldx, Kp, 0, 0, 1, M, K, Kp, 0);
         lo.in = ws + o.xp; lo.ldin = Kp;
     }
-    if (K != Kp || off16(w)) {
+    if (copy.w) {
         pr.copy[pr.ncopy++] = copy_job(w, ws + o.wp, K, Kp, 0, 0, 1, N, K, Kp, 0);
         m.w = (const T*)(ws + o.wp); m.ldw = Kp;
     }
-    if (K != Kp || off16(a)) {
+    if (copy.a) {
         pr.copy[pr.ncopy++] = copy_job(a, ws + o.ap, K, Kp, 0, 0, 1, L * r, K, Kp, 0);
         lo.v = ws + o.ap; lo.ldv = Kp;
     }
@@ -1405,7 +1422,7 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
 template <typename T>
 static int backward_t(const T* dy, const void* x, long long ldx, const unsigned char* exps, const float* t, const T* w, const T* a, const T* b, const float* scale,
                       const int* ids, int M, int K, int N, int r, int L, T* dx, T* da, T* db, char* ws, hipStream_t st) {
-    const BwdWs o = bwd_ws(M, K, N, r, L, sizeof(T));
+    const BwdWs o = bwd_ws(M, K, N, r, L, sizeof(T), dx != nullptr);
     AdArgs<T> g{};
     g.dy = dy; g.w = w; g.a = a; g.b = b; g.scale = scale; g.ids = ids; g.dx = dx; g.u = (float*)(ws + o.u);
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
@@ -1473,7 +1490,13 @@ extern "C" {
 
 size_t hmf_adapted_linear_workspace_bytes(int M, int K, int N, int r, int L, int bf16) {
     if (M < 1 || K < 1 || N < 1 || r < 1 || L < 1) return 0;
-    return fwd_ws(M, K, N, r, L, bf16 ? 2 : 4).total;
+    return fwd_ws(M, K, N, r, L, bf16 ? 2 : 4, kAnyLayout).total;
+}
+
+size_t hmf_adapted_linear_workspace_bytes_for(const void* x, long long ldx, const void* w, const void* a, int M, int K, int N, int r, int L, int bf16) {
+    if (M < 1 || K < 1 || N < 1 || r < 1 || L < 1) return 0;
+    const size_t z = bf16 ? 2 : 4;
+    return fwd_ws(M, K, N, r, L, z, fwd_layout(x, ldx, w, a, K, z)).total;
 }
 
 int hmf_adapted_linear(const void* x, long long ldx, const void* w, const void* bias, const void* a, const void* b, const float* scale, const int* ids, int M, int K,
@@ -1481,7 +1504,7 @@ int hmf_adapted_linear(const void* x, long long ldx, const void* w, const void* 
     if (int rc = check_sizes("hmf_adapted_linear", M, K, N, r, L)) return rc;
     if (M == 0) return HMF_OK;
     if (!x || !w || !a || !b || !scale || !ids || !y || ldx < K) return fail(HMF_ERR_INVALID, "hmf_adapted_linear: null argument or ldx=%lld < K=%d", ldx, K);
-    const size_t need = fwd_ws(M, K, N, r, L, bf16 ? 2 : 4).total;
+    const size_t need = hmf_adapted_linear_workspace_bytes_for(x, ldx, w, a, M, K, N, r, L, bf16);
     if (need && (!workspace || workspace_bytes < need || off16(workspace)))
         return fail(HMF_ERR_WORKSPACE, "hmf_adapted_linear: workspace %zu < %zu bytes (16-byte aligned)", workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;
@@ -1494,7 +1517,12 @@ int hmf_adapted_linear(const void* x, long long ldx, const void* w, const void* 
 
 size_t hmf_adapted_linear_backward_workspace_bytes(int M, int K, int N, int r, int L, int bf16) {
     if (M < 1 || K < 1 || N < 1 || r < 1 || L < 1) return 0;
-    return bwd_ws(M, K, N, r, L, bf16 ? 2 : 4).total;
+    return bwd_ws(M, K, N, r, L, bf16 ? 2 : 4, true).total;
+}
+
+size_t hmf_adapted_linear_backward_workspace_bytes_for(int M, int K, int N, int r, int L, int bf16, int need_dx) {
+    if (M < 1 || K < 1 || N < 1 || r < 1 || L < 1) return 0;
+    return bwd_ws(M, K, N, r, L, bf16 ? 2 : 4, need_dx != 0).total;
 }
 
 int hmf_adapted_linear_backward(const void* dy, const void* x, long long ldx, const unsigned char* exps, const float* t, const void* w, const void* a, const void* b,
@@ -1505,7 +1533,7 @@ int hmf_adapted_linear_backward(const void* dy, const void* x, long long ldx, co
     if (!dy || !x || !t || !w || !a || !b || !scale || !ids || !da || !db || (exps ? ldx != K : ldx < K))
         return fail(HMF_ERR_INVALID, "hmf_adapted_linear_backward: null argument, or ldx=%lld with K=%d (a checkpoint is contiguous)", ldx, K);
     if (off16(dy)) return fail(HMF_ERR_INVALID, "hmf_adapted_linear_backward: dy must be 16-byte aligned");
-    const size_t need = bwd_ws(M, K, N, r, L, bf16 ? 2 : 4).total;
+    const size_t need = bwd_ws(M, K, N, r, L, bf16 ? 2 : 4, dx != nullptr).total;
     if (!workspace || workspace_bytes < need || off16(workspace))
         return fail(HMF_ERR_WORKSPACE, "hmf_adapted_linear_backward: workspace %zu < %zu bytes (16-byte aligned)", workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;

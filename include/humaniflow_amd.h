@@ -415,14 +415,18 @@ int hmf_conv1x1_gemm_avgpool(const float* x, const float* w, const float* bias, 
  * x rows of pitch ldx elements, everything else contiguous; x, w, bias (or NULL), a, b, y all float32, or all bfloat16 with bf16 != 0; sums in 32 bits, one
  * rounding at the end.  t (M, r) float32 is what hmf_adapted_linear_backward takes (NULL: not kept).  M = 0 does nothing; any K, N >= 1; 16-byte aligned
  * rows of a multiple of 16 bytes move 16 bytes per lane.  The workspace (16-byte aligned) needs no initialisation;
- * where none is needed (a few rows) its size is 0 and it may be NULL. */
+ * where none is needed (a few rows) its size is 0 and it may be NULL.  _workspace_bytes: enough for any operands of these sizes; _workspace_bytes_for: what a call
+ * with these very operands needs (many rows of whole aligned chunks of 128 bytes are not copied).  */
 size_t hmf_adapted_linear_workspace_bytes(int M, int K, int N, int r, int L, int bf16);
+size_t hmf_adapted_linear_workspace_bytes_for(const void* x, long long ldx, const void* w, const void* a, int M, int K, int N, int r, int L, int bf16);
 int hmf_adapted_linear(const void* x, long long ldx, const void* w, const void* bias, const void* a, const void* b, const float* scale, const int* ids, int M, int K,
                        int N, int r, int L, int bf16, void* y, float* t, void* workspace, size_t workspace_bytes, void* stream);
 /* Its backward pass, the shared projection held fixed: u[m] = scale[l] b[l]^T dy[m];  dx[m] = w^T dy[m] + a[l]^T u[m] (dx NULL: not computed);
  * da[l] = sum of u[m] x[m]^T over the rows of l, db[l] = sum of dy[m] t[m]^T (an adapter without rows: zeros).  Sums over rows in a fixed order.
- * x: the forward's input, or with exps != NULL the codes of its 8-bit checkpoint (hmf_act8_pack; ldx = K).  dy 16-byte aligned. */
+ * x: the forward's input, or with exps != NULL the codes of its 8-bit checkpoint (hmf_act8_pack; ldx = K).  dy 16-byte aligned.
+ * _workspace_bytes: enough with and without dx; _workspace_bytes_for: what the call needs. */
 size_t hmf_adapted_linear_backward_workspace_bytes(int M, int K, int N, int r, int L, int bf16);
+size_t hmf_adapted_linear_backward_workspace_bytes_for(int M, int K, int N, int r, int L, int bf16, int need_dx);
 int hmf_adapted_linear_backward(const void* dy, const void* x, long long ldx, const unsigned char* exps, const float* t, const void* w, const void* a, const void* b,
                                 const float* scale, const int* ids, int M, int K, int N, int r, int L, int bf16, void* dx, void* da, void* db, void* workspace,
                                 size_t workspace_bytes, void* stream);
