@@ -214,8 +214,9 @@ __global__ __launch_bounds__(256) void k_ad_few(const AdArgs<T> a, int tiles_o, 
 
 // One to four rows (a single image): everything in ONE launch, since a second one costs as much as the work.  A work-group finds the rows' t itself -- A_l is read once per
 // work-group, from L2 -- and then its waves two outputs each, lanes along K.  1 row, 2,048 -> 1,024, rank 16 in 32 bits: 7.6 us, and two launches of 9 us in all in the form below.
-constexpr int kOneRows = 4, kOneBytes = 512 << 10, kOneOdd = 64 << 10;      // rows; bytes of A that a work-group reads for them, and where its rows are not multiples of 4 (4 rows, 1,941 ->
-// 1,379, rank 15: 56 us, 18 below; 4 rows, 1,001 -> 64, rank 8, bfloat16: 16 us, 18 below)
+constexpr int kOneRows = 4, kOneBytes = 512 << 10, kOneOdd = 64 << 10;      // rows; bytes of A that a work-group reads for them, and where it reads them element by
+// element: a width, pitch or address that is no multiple of four elements (4 rows, 1,941 -> 1,379, rank 15: 56 us, 18 below; 2,048 -> 1,024, rank 16, of a wider view: 55 us,
+// 19 below; 4 rows, 1,001 -> 64, rank 8, bfloat16: 16 us, 18 below)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void k_ad_one(const AdArgs<T> a) {
     __shared__ float st[kOneRows][kMaxRank];
@@ -1259,22 +1260,24 @@ static size_t gemm_partial(int M, int O, int Cp, size_t z) {
 // the many-row form's rows: whole chunks of 128 bytes, 16-byte aligned
 static inline int padded(int C, size_t z) { const int bk = (int)(128 / z); return (C + bk - 1) / bk * bk; }
 static inline int rank_pitch(int r) { return (r + 3) & ~3; }
-// one launch for one to four rows: a rule on the sizes alone, so that its callers need no workspace (an allocation is 1.3 us of 12)
-static inline bool one_launch(int M, int K, int r, size_t z) {
-    return M <= kOneRows && (long long)M * r * K * (int)z <= (K % 4 == 0 ? kOneBytes : kOneOdd);
-}
-// how the forward's operands lie: which of them the many-row form has to copy into whole chunks of aligned rows
-struct FwdLayout { bool x, w, a; };
-constexpr FwdLayout kAnyLayout{true, true, true};
+// how the forward's operands lie: which of them the many-row form has to copy into whole chunks of aligned rows, and whether the few-row forms can read four elements at a
+// time (load4's VEC)
+struct FwdLayout { bool x, w, a, vec; };
+constexpr FwdLayout kAnyLayout{true, true, true, false};
 static FwdLayout fwd_layout(const void* x, long long ldx, const void* w, const void* a, int K, size_t z) {
     const bool odd = K != padded(K, z);
-    return {odd || ldx % (long long)(16 / z) != 0 || off16(x), odd || off16(w), odd || off16(a)};
+    return {odd || ldx % (long long)(16 / z) != 0 || off16(x), odd || off16(w), odd || off16(a),
+            K % 4 == 0 && ldx % 4 == 0 && !(((uintptr_t)x | (uintptr_t)w | (uintptr_t)a) & (4 * z - 1))};
+}
+// one launch for one to four rows: no workspace (an allocation is 1.3 us of 12)
+static inline bool one_launch(int M, int K, int r, size_t z, bool vec) {
+    return M <= kOneRows && (long long)M * r * K * (int)z <= (vec ? kOneBytes : kOneOdd);
 }
 struct FwdWs { size_t t, partial, order, key, seg, xp, wp, ap, total; };
-static FwdWs fwd_ws(int M, int K, int N, int r, int L, size_t z, const FwdLayout& copy) {
+static FwdWs fwd_ws(int M, int K, int N, int r, int L, size_t z, const FwdLayout& in) {
     FwdWs w{};
     size_t o = 0;
-    if (one_launch(M, K, r, z)) return w;
+    if (one_launch(M, K, r, z, in.vec)) return w;
     w.t = o; o += al((size_t)M * rank_pitch(r) * 4);
     if (M <= kFewRows) {
         int ks, kw;
@@ -1285,9 +1288,9 @@ static FwdWs fwd_ws(int M, int K, int N, int r, int L, size_t z, const FwdLayout
         w.order = o; o += al((size_t)M * 4);
         w.key = o; o += al((size_t)M * 4);
         w.seg = o; o += al((size_t)(L + 2) * 4);
-        w.xp = o; o += copy.x ? al(M * Kp * z) : 0;
-        w.wp = o; o += copy.w ? al(N * Kp * z) : 0;
-        w.ap = o; o += copy.a ? al((size_t)L * r * Kp * z) : 0;
+        w.xp = o; o += in.x ? al(M * Kp * z) : 0;
+        w.wp = o; o += in.w ? al(N * Kp * z) : 0;
+        w.ap = o; o += in.a ? al((size_t)L * r * Kp * z) : 0;
         w.partial = o; o += al(gemm_partial(M, N, (int)Kp, z));
     }
     w.total = o;
@@ -1364,15 +1367,14 @@ template <typename T> static int gemm(AdGemm<T>& m, void* partial, hipStream_t s
 template <typename T>
 static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const T* a, const T* b, const float* scale, const int* ids, int M, int K, int N, int r, int L,
                      T* y, float* t, char* ws, hipStream_t st) {
-    const FwdLayout copy = fwd_layout(x, ldx, w, a, K, sizeof(T));
-    const FwdWs o = fwd_ws(M, K, N, r, L, sizeof(T), copy);
+    const FwdLayout in = fwd_layout(x, ldx, w, a, K, sizeof(T));
+    const FwdWs o = fwd_ws(M, K, N, r, L, sizeof(T), in);
     AdArgs<T> g{};
     g.x = x; g.ldx = ldx; g.w = w; g.bias = bias; g.a = a; g.b = b; g.scale = scale; g.ids = ids; g.y = y; g.t = t ? t : (float*)(ws + o.t);
     g.M = M; g.K = K; g.N = N; g.r = r; g.L = L;
-    const bool vec = K % 4 == 0 && ldx % 4 == 0 && !(((uintptr_t)x | (uintptr_t)w | (uintptr_t)a) & (4 * sizeof(T) - 1));      // load4's; few rows
-    if (one_launch(M, K, r, sizeof(T))) {
+    if (one_launch(M, K, r, sizeof(T), in.vec)) {
         g.t = t;
-        if (vec) hipLaunchKernelGGL((k_ad_one<T, true>), dim3(blocks_of(N, 8)), dim3(256), 0, st, g);
+        if (in.vec) hipLaunchKernelGGL((k_ad_one<T, true>), dim3(blocks_of(N, 8)), dim3(256), 0, st, g);
         else hipLaunchKernelGGL((k_ad_one<T, false>), dim3(blocks_of(N, 8)), dim3(256), 0, st, g);
         HMF_LAUNCH_CHECK();
         return HMF_OK;
@@ -1382,7 +1384,7 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
         g.partial = (float*)(ws + o.partial);
         const int to = blocks_of(N, 32), tm = blocks_of(M, 32);
         const dim3 grid(to * g.ksplit * tm + M);
-        if (vec) hipLaunchKernelGGL((k_ad_few<T, true>), grid, dim3(256), 0, st, g, to, tm);
+        if (in.vec) hipLaunchKernelGGL((k_ad_few<T, true>), grid, dim3(256), 0, st, g, to, tm);
         else hipLaunchKernelGGL((k_ad_few<T, false>), grid, dim3(256), 0, st, g, to, tm);
         HMF_LAUNCH_CHECK();
         hipLaunchKernelGGL(k_ad_join<T>, dim3(blocks_of((long long)M * N, 64)), dim3(64), 0, st, g);
@@ -1397,15 +1399,15 @@ static int forward_t(const T* x, long long ldx, const T* w, const T* bias, const
     lo.in = x; lo.ldin = ldx; lo.v = a; lo.ldv = K;
     AdGemm<T> m{};
     m.w = w; m.ldw = K;
-    if (copy.x) {
+    if (in.x) {
         pr.copy[pr.ncopy++] = copy_job(x, ws + o.xp, ldx, Kp, 0, 0, 1, M, K, Kp, 0);
         lo.in = ws + o.xp; lo.ldin = Kp;
     }
-    if (copy.w) {
+    if (in.w) {
         pr.copy[pr.ncopy++] = copy_job(w, ws + o.wp, K, Kp, 0, 0, 1, N, K, Kp, 0);
         m.w = (const T*)(ws + o.wp); m.ldw = Kp;
     }
-    if (copy.a) {
+    if (in.a) {
         pr.copy[pr.ncopy++] = copy_job(a, ws + o.ap, K, Kp, 0, 0, 1, L * r, K, Kp, 0);
         lo.v = ws + o.ap; lo.ldv = Kp;
     }

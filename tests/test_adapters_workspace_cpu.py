@@ -40,3 +40,14 @@ def test_backward_holds_partial_sums_of_adapters_with_many_rows_only(lib, bf16):
     assert size(4096, 16, 1) > size(4096, 16, 0) and size(200, 16, 1) > size(200, 16, 0)
     for M, L in ((4096, 16), (200, 16)):
         assert lib.hmf_adapted_linear_backward_workspace_bytes(M, 2048, 1024, 16, L, bf16) == size(M, L, 1)
+
+
+@pytest.mark.parametrize('bf16', [0, 1])
+def test_one_launch_goes_by_how_the_operands_lie(lib, bf16):
+    """Four rows and 256 or 512 KB of A are one launch (no workspace) only where four elements are read at a time; up to 64 KB always."""
+    z = 2 if bf16 else 4
+    size = lambda x=A16, ldx=2048, w=A16, a=A16, K=2048, r=16, M=4: lib.hmf_adapted_linear_workspace_bytes_for(x, ldx, w, a, M, K, 1024, r, 3, bf16)
+    assert size() == 0 and size(ldx=2052) == 0 and size(x=A16 + 4 * z) == 0
+    assert size(ldx=2049) > 0 and size(x=A16 + z) > 0 and size(w=A16 + z) > 0 and size(a=A16 + z) > 0 and size(K=2047) > 0
+    assert size(ldx=2049, r=1) == 0 and size(K=2047, ldx=2047, r=1) == 0 and size(M=5) > 0
+    assert lib.hmf_adapted_linear_workspace_bytes(4, 2048, 1024, 16, 3, bf16) == size(ldx=2049)      # enough for any operands

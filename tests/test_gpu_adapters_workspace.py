@@ -95,3 +95,21 @@ def test_many_adapters_do_not_cost_memory():
     for need_dx in (True, False):
         out, held = extra(lambda: adapters.adapted_linear_backward(dy, x, t, w, A, B, scale, ids, need_dx=need_dx))
         assert held - size(*out) < size(B) + size(w) + (8 << 20)             # partial sums of every adapter: 396 MB
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('M', [1, 2, 4])
+def test_few_rows_of_a_wider_view(M, dtype):
+    """2,048 -> 1,024 at rank 16: rows of an odd pitch and an odd start, and an A that starts between four elements."""
+    K, N, r, L = 2048, 1024, 16, 3
+    g = torch.Generator().manual_seed(M)
+    rn = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()
+    x, w, B = rn(M, K + 3)[:, 1:K + 1], rn(N, K) / K ** 0.5, rn(L, N, r)
+    A = (rn(L * r * K + 1) / K ** 0.5)[1:].view(L, r, K)
+    scale, ids = (0.5 + torch.rand(L, generator=g)).cuda(), torch.tensor([2, 0, -1, 1], dtype=torch.int32, device='cuda')[:M].contiguous()
+    for a in (A, A.clone()):
+        for v in (x, x.contiguous()):
+            y, t = adapters.adapted_linear_forward(v, w, None, a, B, scale, ids)
+            ry, rt, ey, et = oad.forward(_d(x), _d(w), None, _d(A), _d(B), _d(scale), ids.cpu().numpy())
+            _near(y, ry, ey)
+            _near(t, rt, et)
