@@ -135,16 +135,16 @@ class _AdaptedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, A, B, scale, ids, checkpoint):
         y, t = adapted_linear_forward(x, weight, bias, A, B, scale, ids)
-        ctx.ck = act8.pack(x) if checkpoint == 'int8' else None            # then x itself is not kept
-        ctx.save_for_backward(x if ctx.ck is None else None, t, weight, A, B, scale, ids)
+        ck = act8.pack(x) if checkpoint == 'int8' else None                 # with a checkpoint x itself is not kept
+        ctx.save_for_backward(x if ck is None else None, t, weight, A, B, scale, ids, *((None, None) if ck is None else (ck.codes, ck.exps)))
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, t, weight, A, B, scale, ids = ctx.saved_tensors
-        if ctx.ck is not None:
-            x = ctx.ck
+        x, t, weight, A, B, scale, ids, codes, exps = ctx.saved_tensors
+        if codes is not None:
+            x = act8.Act8(codes, exps)
         dx, dA, dB = adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=ctx.needs_input_grad[0])
         return dx, None, None, dA, dB, None, None, None
 
