@@ -135,7 +135,7 @@ class _AdaptedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, A, B, scale, ids, checkpoint):
         y, t = adapted_linear_forward(x, weight, bias, A, B, scale, ids)
-        ck = act8.pack(x) if checkpoint == 'int8' else None                 # with a checkpoint x itself is not kept
+        ck = act8.pack(x) if checkpoint == 'int8' else checkpoint           # with a checkpoint x itself is not kept
         ctx.save_for_backward(x if ck is None else None, t, weight, A, B, scale, ids, *((None, None) if ck is None else (ck.codes, ck.exps)))
         return y
 
@@ -151,10 +151,13 @@ class _AdaptedLinear(torch.autograd.Function):
 
 def adapted_linear(x, weight, bias, A, B, scale, ids, checkpoint=None):
     """y (M, N).  Differentiable w.r.t. x, A and B; the shared projection is held fixed (a weight, bias or scale that requires a gradient is refused).
-    checkpoint='int8': the backward pass keeps x in 8 bits.  To capture forward and backward into a HIP graph, first let go of every eager pass over the same
-    parameters (its outputs and loss)."""
-    if checkpoint not in (None, 'int8'):
-        raise ValueError("humaniflow_amd: checkpoint must be None or 'int8', got %r" % (checkpoint,))
+    checkpoint='int8': the backward pass keeps x in 8 bits; act8.pack(x) in its place is kept as it is, so that layers which read the same x share one.  To capture forward
+    and backward into a HIP graph, first let go of every eager pass over the same parameters (its outputs and loss)."""
+    if isinstance(checkpoint, act8.Act8):
+        if checkpoint.shape != x.shape or checkpoint.device != x.device:
+            raise ValueError('humaniflow_amd: the checkpoint holds %s rows on %s, x is %s on %s' % (tuple(checkpoint.shape), checkpoint.device, tuple(x.shape), x.device))
+    elif checkpoint not in (None, 'int8'):
+        raise ValueError("humaniflow_amd: checkpoint must be None, 'int8' or an Act8 of x, got %r" % (checkpoint,))
     if torch.is_grad_enabled():
         if weight.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad):
             raise RuntimeError('humaniflow_amd: adapters are fitted beside a fixed projection: call requires_grad_(False) on its weight and bias, and on scale')
@@ -188,8 +191,14 @@ class LowRankAdapters(nn.Module):
             self.register_parameter(name + '_A', nn.Parameter(A))
             self.register_parameter(name + '_B', nn.Parameter(torch.zeros(num_adapters, lin.out_features, rank, dtype=torch.float32, device=ref.device)))
 
-    def linear(self, name, lin, x, ids):
+    def keep(self, x, names):
+        """The 8-bit checkpoint of x that the layers `names`, which all read it, share (linear's `kept`), or None where the option is off or nothing is differentiated."""
+        if self.checkpoint is None or not torch.is_grad_enabled() or not any(n in self.layers for n in names):
+            return None
+        return act8.pack(x) if x.requires_grad or any(p.requires_grad for p in self.parameters()) else None
+
+    def linear(self, name, lin, x, ids, kept=None):
         """lin(x) with the rows' own adapters, or lin(x) alone for a layer that has none."""
         if name not in self.layers:
             return torch.nn.functional.linear(x, lin.weight, lin.bias)
-        return adapted_linear(x, lin.weight, lin.bias, getattr(self, name + '_A'), getattr(self, name + '_B'), self.scale, ids, self.checkpoint)
+        return adapted_linear(x, lin.weight, lin.bias, getattr(self, name + '_A'), getattr(self, name + '_B'), self.scale, ids, self.checkpoint if kept is None else kept)

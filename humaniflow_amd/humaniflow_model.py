@@ -679,11 +679,12 @@ class HumaniflowModel(nn.Module):
         nb, P, N = self.num_shape_params, self.num_bodyparts, int(num_samples)
 
         if adapter_ids is not None:                                                      # :232-253 with every image's own adapters (adapters.py)
-            head = lambda name, v: self.adapters.linear(name, getattr(self, name), v, adapter_ids)
+            head = lambda name, v, kept=None: self.adapters.linear(name, getattr(self, name), v, adapter_ids, kept)
             x = self.activation(head('fc1', input_feats.to(torch.float32)))
-            cam = head('fc_cam', x) + self.init_cam
-            glob_R = rot6d_to_rotmat(head('fc_glob', x) + self.init_glob)
-            shape_params = head('fc_shape', x)
+            kept = self.adapters.keep(x, ('fc_cam', 'fc_glob', 'fc_shape'))
+            cam = head('fc_cam', x, kept) + self.init_cam
+            glob_R = rot6d_to_rotmat(head('fc_glob', x, kept) + self.init_glob)
+            shape_params = head('fc_shape', x, kept)
             shape_mode, shape_log_std = shape_params[:, :nb], shape_params[:, nb:]
             shape_std = torch.exp(shape_log_std)
         elif (grad and self.heads_kernel and batch_size <= 128 and isinstance(self.activation, torch.nn.ELU) and self._heads_kernel_supports(input_feats)):
