@@ -495,13 +495,14 @@ PER_FRAME_MODEL_KEYS = ('glob_rotmat', 'pose_rotmats_point_est', 'shape_mode', '
 
 
 @torch.no_grad()
-def predict_batch(model, smpl, batch, num_samples, noise=None, materialise_tpose=True):
+def predict_batch(model, smpl, batch, num_samples, noise=None, materialise_tpose=True, adapter_ids=None):
     """evaluate/evaluate_humaniflow.py:113-192 on the device: model -> SMPL point estimate + samples (ONE launch of B*N + B bodies) ->
     the evaluation joints, COCO joints and their 2-D projection of all rows (one launch, hmf_eval_joints) -> T-pose bodies of both (one
     launch).  materialise_tpose=False: the T-pose bodies are not built; the dict carries `tpose_betas` (B, nb) / `tpose_betas_samples`
-    (B, N, nb) instead and an EvalMetricsTracker(smpl=...) scores them with hmf_smpl_tpose_errors (no 2 x 267 MB vertex round trip)."""
+    (B, N, nb) instead and an EvalMetricsTracker(smpl=...) scores them with hmf_smpl_tpose_errors (no 2 x 267 MB vertex round trip).
+    adapter_ids (B,): each image's own low-rank adapter of the model's heads (HumaniflowModel.attach_adapters); without it attached adapters are left out."""
     N = num_samples
-    pred = model(batch['input'], num_samples=N, noise=noise)
+    pred = model(batch['input'], num_samples=N, noise=noise, adapter_ids=adapter_ids)
     g = pred['glob_rotmat']
     B = g.shape[0]
     img_wh = batch['input'].shape[-1]

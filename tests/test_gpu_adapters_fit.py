@@ -61,3 +61,20 @@ def test_gradients_through_a_fixed_flow_are_those_through_a_trained_one():
         got[fixed] = {n: p.grad.double().clone() for n, p in model.adapters.named_parameters()}
     for n, g in got[True].items():
         assert g.norm() > 0 and (g - got[False][n]).norm() <= 1e-4 * got[False][n].norm(), n
+
+
+@pytest.mark.parametrize('N', [0, 2])
+def test_evaluation_takes_each_images_adapter(N):
+    """evaluate.predict_batch with adapter_ids: each image's outputs are those of the model with its adapter, and without ids those of the model alone."""
+    from humaniflow_amd import evaluate as ev
+    _, model, smpl, _, _ = _setup(3)
+    batch = ev.SyntheticEvalSet(3, size=128, seed=1).batch([0, 1, 2], torch.device('cuda'))
+    noise = {'shape': torch.randn(N, 3, 10, device='cuda'), 'pose': torch.randn(23, 3, N, 3, device='cuda')} if N else None
+    ids = torch.tensor([1, -1, 2], device='cuda')
+    got, plain = (ev.predict_batch(model, smpl, batch, N, noise=noise, adapter_ids=i) for i in (ids, None))
+    with torch.no_grad():
+        ref = model(batch['input'], num_samples=N, noise=noise, adapter_ids=ids)
+    for k in ev.PER_FRAME_MODEL_KEYS:
+        assert torch.equal(got[k], ref[k])
+    moved = (got['verts3D'] - plain['verts3D']).abs().amax(dim=(1, 2))
+    assert moved[0] > 1e-4 and moved[2] > 1e-4 and moved[1] < 1e-5
