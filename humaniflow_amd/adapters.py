@@ -76,7 +76,8 @@ def adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t=True):
     if x.dtype != weight.dtype:
         raise ValueError('humaniflow_amd: adapted_linear: x is %s, the weight %s' % (x.dtype, weight.dtype))
     x, ldx = _rows(x)
-    weight, bias, A, B, scale = _dense(weight), _dense(bias), _dense(A), _dense(B), _dense(scale)
+    if not (weight.is_contiguous() and A.is_contiguous() and B.is_contiguous() and scale.is_contiguous() and (bias is None or bias.is_contiguous())):
+        weight, bias, A, B, scale = _dense(weight), _dense(bias), _dense(A), _dense(B), _dense(scale)
     dev = weight.device
     st = _lib.stream_here(dev)
     if st is None:
@@ -86,10 +87,10 @@ def adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t=True):
     t = torch.empty((M, r), dtype=torch.float32, device=dev) if need_t else None
     lib = _lib.load()
     bf16 = int(weight.dtype == torch.bfloat16)
-    n = lib.hmf_adapted_linear_workspace_bytes_for(x.data_ptr(), ldx, weight.data_ptr(), A.data_ptr(), M, K, N, r, L, bf16)
+    xp, wp, ap = x.data_ptr(), weight.data_ptr(), A.data_ptr()
+    n = lib.hmf_adapted_linear_workspace_bytes_for(xp, ldx, wp, ap, M, K, N, r, L, bf16)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None      # a few rows need none
-    _lib.check(lib.hmf_adapted_linear(x.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(), A.data_ptr(), B.data_ptr(), scale.data_ptr(),
-                                      ids.data_ptr(), M, K, N, r, L, bf16, y.data_ptr(), None if t is None else t.data_ptr(), None if ws is None else ws.data_ptr(), n, st), 'hmf_adapted_linear')
+    _lib.check(lib.hmf_adapted_linear(xp, ldx, wp, None if bias is None else bias.data_ptr(), ap, B.data_ptr(), scale.data_ptr(), ids.data_ptr(), M, K, N, r, L, bf16, y.data_ptr(), None if t is None else t.data_ptr(), None if ws is None else ws.data_ptr(), n, st), 'hmf_adapted_linear')
     return y, t
 
 
@@ -107,7 +108,8 @@ def adapted_linear_backward(dy, x, t, weight, A, B, scale, ids, need_dx=True):
     dy = _dense(dy)
     if dy.data_ptr() % 16:
         dy = dy.clone()
-    t, weight, A, B, scale = _dense(t), _dense(weight), _dense(A), _dense(B), _dense(scale)
+    if not (t.is_contiguous() and weight.is_contiguous() and A.is_contiguous() and B.is_contiguous() and scale.is_contiguous()):
+        t, weight, A, B, scale = _dense(t), _dense(weight), _dense(A), _dense(B), _dense(scale)
     if M == 0:
         return (torch.empty((0, K), dtype=dt, device=dev) if need_dx else None), torch.zeros_like(A), torch.zeros_like(B)
     if kept8:
