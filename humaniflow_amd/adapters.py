@@ -45,8 +45,9 @@ def _check(x, weight, bias, A, B, scale, ids):
         raise ValueError('humaniflow_amd: `ids` must be int32 or int64 (%d), got %s %s' % (M, ids.dtype, tuple(ids.shape)))
     if not weight.is_cuda:
         _lib.require_cuda(weight, 'weight')
-    dev = weight.device
-    if x.device != dev or A.device != dev or B.device != dev or scale.device != dev or ids.device != dev or (bias is not None and bias.device != dev):
+    dev, at = weight.device, weight.get_device()                             # numbers compare in half the time of devices, and this is a small call's host time
+    if (x.device != dev or A.get_device() != at or B.get_device() != at or scale.get_device() != at or ids.get_device() != at
+            or (bias is not None and bias.get_device() != at)):
         for name, t in (('x', x), ('bias', bias), ('A', A), ('B', B), ('scale', scale), ('ids', ids)):
             if t is not None and t.device != dev:
                 raise ValueError('humaniflow_amd: `%s` is on %s, the weight on %s' % (name, t.device, dev))
