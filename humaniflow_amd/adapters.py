@@ -5,8 +5,9 @@
     y = adapted_linear(x, weight, bias, A, B, scale, ids)                        differentiable w.r.t. x, A and B (the shared projection is held fixed)
     y, t = adapted_linear_forward(...);  dx, dA, dB = adapted_linear_backward(dy, x, t, weight, A, B, scale, ids)
 
-x (M, K), weight (N, K), bias (N) or None, A (L, r, K), B (L, N, r): all float32 or all bfloat16; scale (L) float32; ids (M) int32 / int64; r <= 64.  An id of L or
-more has no adapter to go with: that row's outputs are NaN.  The backward pass takes x as it was or as an 8-bit checkpoint (act8.Act8).
+x (M, K), weight (N, K), bias (N) or None, A (L, r, K), B (L, N, r): all float32 or all bfloat16; scale (L) float32; ids (M) int32 / int64; r <= 64,
+L + M / 256 <= 65,535 and M max(K, N) up to some 1.7e10.  An id of L or more has no adapter to go with: that row's outputs
+are NaN.  The backward pass takes x as it was or as an 8-bit checkpoint (act8.Act8).
 `LowRankAdapters` holds the adapters of a HumaniflowModel's heads (models/humaniflow_model.py:232-252): `model.attach_adapters(...)`, then
 `model(..., adapter_ids=ids)`.  Kernels: csrc/adapters.hip.
 """

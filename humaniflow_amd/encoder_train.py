@@ -22,7 +22,8 @@ Filter re-layouts (flip, transpose, channels_last) are small torch copies per st
 
 With `ResNetEncoder.activation_checkpoint = 'int8'` a unit keeps its y as an 8-bit checkpoint and one ReLU bit per element (act8.py) and, where an identity was
 added, its out as a second one, instead of both in 32 bits: the BatchNorm backward reads the checkpoint (hmf_bn_backward_act8), the weight gradient's input is
-rebuilt from it one unit at a time.  The forward's values are the same; the gradients carry the 8-bit rounding of what was kept.
+rebuilt from it one unit at a time (with WGRAD_SIDE_STREAM they are all held to the end of the backward pass).  A unit's forward values are the same bits;
+the gradients carry the 8-bit rounding of what was kept.
 """
 import os
 
