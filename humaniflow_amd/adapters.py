@@ -15,7 +15,7 @@ import torch
 from torch import nn
 
 from . import _lib, act8
-from .autograd import refuse_capture_beside_default_stream_pass
+from .autograd import leaves_of, note_stream, refuse_capture_beside_default_stream_pass
 
 MAX_RANK = 64
 
@@ -167,7 +167,9 @@ def adapted_linear(x, weight, bias, A, B, scale, ids, checkpoint=None):
             raise RuntimeError('humaniflow_amd: adapters are fitted beside a fixed projection: call requires_grad_(False) on its weight and bias, and on scale')
         if x.requires_grad or A.requires_grad or B.requires_grad:
             y = _AdaptedLinear.apply(x, weight, bias, A, B, scale, ids, checkpoint)
-            refuse_capture_beside_default_stream_pass([n for n, _ in y.grad_fn.next_functions if hasattr(n, 'variable')], y.device, 'adapted_linear')
+            leaves = leaves_of(y.grad_fn)
+            note_stream(leaves, y.device)
+            refuse_capture_beside_default_stream_pass(leaves, 'adapted_linear')
             return y
     return adapted_linear_forward(x, weight, bias, A, B, scale, ids, need_t=False)[0]
 

@@ -36,17 +36,25 @@ def _atb(A, B, batch, rows, m, n, lda, ldb, sA, sB, want_sum):
     return Cm, sm
 
 
-def refuse_capture_beside_default_stream_pass(nodes, device, what):
-    """A leaf's gradient is added on the stream on which its first living graph was built.  If that is the legacy default stream and this graph is being captured into
-    a HIP graph, the captured backward pass would have to wait for a stream that no capture can hold, which ends the process: refused here instead.
-    nodes: the leaves' nodes in the graph just built; what is noted on one lives as long as a graph of its leaf does."""
-    capturing = torch.cuda.is_current_stream_capturing()
-    for node in nodes:
-        if not capturing:
+def leaves_of(node):
+    """The nodes that add the gradients of `node`'s leaves."""
+    return [n for n, _ in node.next_functions if hasattr(n, 'variable')]
+
+
+def note_stream(nodes, device):
+    """A leaf's gradient is added on the stream on which its first living graph was built: noted on the leaves' nodes of a graph just built eagerly.  The note lives as
+    long as a graph of its leaf does."""
+    if not torch.cuda.is_current_stream_capturing():
+        for node in nodes:
             node.metadata.setdefault('hmf_stream', torch._C._cuda_getCurrentRawStream(device.index))
-        elif node.metadata.get('hmf_stream') == 0:
-            raise RuntimeError('humaniflow_amd: %s is captured while a pass over the same parameters, run eagerly on the default stream, is still '
-                               'alive: let go of its outputs and loss first (del), or run it on another stream' % what)
+
+
+def refuse_capture_beside_default_stream_pass(nodes, what):
+    """If that is the legacy default stream and this pass is being captured into a HIP graph, the captured backward pass would have to wait for a stream that no capture
+    can hold, which ends the process: refused instead."""
+    if torch.cuda.is_current_stream_capturing() and any(node.metadata.get('hmf_stream') == 0 for node in nodes):
+        raise RuntimeError('humaniflow_amd: %s is captured while a pass over the same parameters, run eagerly on the default stream, is still '
+                           'alive: let go of its outputs and loss first (del), or run it on another stream' % what)
 
 
 # ---- records of the flow backward kernels ---------------------------------------------------------------------------------

@@ -469,10 +469,9 @@ class ResNetEncoder(nn.Module):
         if self.training and wants_grad and not x.requires_grad and self.conv1.in_channels == 18:
             # training step: batch-statistics BatchNorm forward + full backward on the library's kernels (encoder_train.py)
             from .encoder_train import EncoderTrainFn
-            from .autograd import refuse_capture_beside_default_stream_pass
+            from .autograd import leaves_of, note_stream
             feats = EncoderTrainFn.apply(self, x, *list(self.parameters()))
-            leaf = next(n for n, _ in feats.grad_fn.next_functions if hasattr(n, 'variable'))      # every pass holds all of them: one leaf speaks for the others
-            refuse_capture_beside_default_stream_pass([leaf], feats.device, 'the encoder\'s training pass')
+            note_stream(leaves_of(feats.grad_fn)[:1], feats.device)         # every pass holds all of the leaves: one speaks for the others
             return feats
         # remaining combinations (train() without gradients, eval() with gradients = frozen statistics under autograd, gradients w.r.t. the
         # input) have no hand-written path and there is no vendor-library path in the product: fail loudly.  (`forward_module` is the plain

@@ -30,6 +30,7 @@ import os
 import torch
 
 from . import _lib, act8
+from .autograd import leaves_of, refuse_capture_beside_default_stream_pass
 
 CL = torch.channels_last
 WINOGRAD_WGRAD = True          # stride-1 3x3 weight gradients on hmf_conv_wgrad_winograd where the shape is built (False: hmf_conv_wgrad everywhere)
@@ -548,6 +549,7 @@ class EncoderTrainFn(torch.autograd.Function):
         if ctx.saved is None:
             raise RuntimeError('humaniflow_amd: the encoder training graph was already back-propagated; its saved activations are freed after the '
                                'first backward (retain_graph is not supported for EncoderTrainFn)')
+        refuse_capture_beside_default_stream_pass(leaves_of(ctx)[:1], 'the encoder\'s backward pass')
         for p, v in zip(ctx.params_ref, ctx.param_versions):
             if p._version != v:
                 raise RuntimeError('humaniflow_amd: an encoder parameter was modified in place between the forward and the backward of the training '
