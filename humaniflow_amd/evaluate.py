@@ -502,7 +502,7 @@ def predict_batch(model, smpl, batch, num_samples, noise=None, materialise_tpose
     (B, N, nb) instead and an EvalMetricsTracker(smpl=...) scores them with hmf_smpl_tpose_errors (no 2 x 267 MB vertex round trip).
     adapter_ids (B,): each image's own low-rank adapter of the model's heads (HumaniflowModel.attach_adapters); without it attached adapters are left out."""
     N = num_samples
-    pred = model(batch['input'], num_samples=N, noise=noise, adapter_ids=adapter_ids)
+    pred = model(batch['input'], num_samples=N, noise=noise, **({} if adapter_ids is None else {'adapter_ids': adapter_ids}))
     g = pred['glob_rotmat']
     B = g.shape[0]
     img_wh = batch['input'].shape[-1]

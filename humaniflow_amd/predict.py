@@ -27,7 +27,7 @@ def predict_humaniflow(humaniflow_model, smpl_model, proxy_inputs, names, save_d
         x = proxy_inputs[i:i + 1]
         nz = None if noise is None else {k: v[:, i:i + 1].contiguous() for k, v in noise.items()}
         pred = humaniflow_model(x, num_samples=N, use_shape_mode_for_samples=True, return_input_feats=True, noise=nz,   # :112-115
-                                adapter_ids=None if adapter_ids is None else adapter_ids[i:i + 1])
+                                **({} if adapter_ids is None else {'adapter_ids': adapter_ids[i:i + 1]}))
         out_np = {k: pred[k].cpu().numpy()[0] for k in ('pose_axisangle_point_est', 'pose_rotmats_point_est', 'shape_mode',
                                                           'glob_rotmat', 'cam_wp', 'input_feats')}          # predict_utils.py:19-24
         if save_dir is not None:

@@ -59,7 +59,7 @@ def train_forward_loss(model, smpl, criterion, proxy_input, targets, num_samples
     N = num_samples
     pred = model(proxy_input, compute_point_est=True, num_samples=N, compute_for_loglik=True, shape_for_loglik=targets['shape'],
                  pose_R_for_loglik=targets['pose_rotmats'], glob_R_for_loglik=targets['glob_rotmats'], noise=noise, input_feats=input_feats,
-                 adapter_ids=adapter_ids)
+                 **({} if adapter_ids is None else {'adapter_ids': adapter_ids}))
     B = pred['glob_rotmat'].shape[0]
     cfg_l = criterion.loss_cfg
     dists = pred['conditioned_pose_SO3flow_dists_for_loglik']
