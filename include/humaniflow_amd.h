@@ -414,9 +414,10 @@ int hmf_conv1x1_gemm_avgpool(const float* x, const float* w, const float* bias, 
  *   t[m] = scale[l] a[l] x[m]      y[m] = w x[m] + bias + b[l] t[m]          w (N, K), a (L, r, K), b (L, N, r), scale (L), r <= 64
  * x rows of pitch ldx elements, everything else contiguous; x, w, bias (or NULL), a, b, y all float32, or all bfloat16 with bf16 != 0; sums in 32 bits, one
  * rounding at the end.  t (M, r) float32 is what hmf_adapted_linear_backward takes (NULL: not kept).  M = 0 does nothing; any K, N >= 1; L + M / 256 <=
- * 65,535 and grids of under 2^32 threads (M max(K, N) up to some 1.7e10), else HMF_ERR_UNSUPPORTED; 16-byte aligned rows of a multiple of 16 bytes move 16 bytes per lane.  The workspace (16-byte aligned) needs no initialisation;
- * where none is needed (a few rows) its size is 0 and it may be NULL.  _workspace_bytes: enough for any operands of these sizes; _workspace_bytes_for: what a call
- * with these very operands needs (many rows of whole aligned chunks of 128 bytes are not copied).  */
+ * 65,535 and grids of under 2^32 threads (M max(K, N) up to some 1.7e10), else HMF_ERR_UNSUPPORTED; 16-byte aligned rows of a multiple of 16 bytes move 16
+ * bytes per lane.  The workspace (16-byte aligned) needs no initialisation; where none is needed (a few rows) its size is 0 and it may be NULL.
+ * _workspace_bytes: enough for any operands of these sizes; _workspace_bytes_for: what a call with these very operands needs (many rows of whole aligned chunks of
+ * 128 bytes are not copied). */
 size_t hmf_adapted_linear_workspace_bytes(int M, int K, int N, int r, int L, int bf16);
 size_t hmf_adapted_linear_workspace_bytes_for(const void* x, long long ldx, const void* w, const void* a, int M, int K, int N, int r, int L, int bf16);
 int hmf_adapted_linear(const void* x, long long ldx, const void* w, const void* bias, const void* a, const void* b, const float* scale, const int* ids, int M, int K,
