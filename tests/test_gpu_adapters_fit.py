@@ -78,3 +78,41 @@ def test_evaluation_takes_each_images_adapter(N):
         assert torch.equal(got[k], ref[k])
     moved = (got['verts3D'] - plain['verts3D']).abs().amax(dim=(1, 2))
     assert moved[0] > 1e-4 and moved[2] > 1e-4 and moved[1] < 1e-5
+
+
+@pytest.mark.parametrize('ids_type', [torch.int32, torch.int64])
+def test_captured_training_pass_of_adapters_and_encoder(ids_type):
+    """Loss and gradients of a whole training pass -- encoder with 8-bit checkpoints, adapted heads, flow, body model -- in one graph, replayed with other images, ids and
+    adapters between the program's own passes.  Some weight gradients are summed by float atomics: within 1e-4 of their norm, as in the encoder's own test."""
+    cfg, model, smpl, batch, _ = _setup(checkpoint='int8')
+    model.image_encoder.requires_grad_(True).train()
+    model.image_encoder.activation_checkpoint = 'int8'
+    crit = H.HumaniflowLoss(cfg.LOSS, 128)
+    params = [p for p in model.parameters() if p.requires_grad]
+    noise = {'shape': torch.randn(2, 4, 10, device='cuda'), 'pose': torch.randn(23, 4, 2, 3, device='cuda')}
+    ids = torch.tensor([0, 1, -1, 2], device='cuda').to(ids_type)
+
+    def step():
+        loss, _ = T.train_forward_loss(model, smpl, crit, batch[0], batch[1], 2, noise=noise, adapter_ids=ids)
+        return [loss.detach(), *torch.autograd.grad(loss, params)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(3):
+        with torch.no_grad():
+            batch[0].copy_(torch.rand_like(batch[0]))
+            ids.copy_(torch.randint(-1, 3, (4,), device='cuda'))
+            model.adapters.fc1_A.mul_(1.1)
+            noise['pose'].mul_(0.9)
+        graph.replay()
+        got = [t.clone() for t in held]
+        want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert (a.double() - b.double()).norm().item() <= 1e-4 * b.double().norm().item() + 1e-12, k
